@@ -220,7 +220,7 @@ def prepare(case, seed):
         if case["state"]:
             slots = [torch.randint(0, 256, (4, case["state"]), generator=gen, device=dev, dtype=torch.uint8)]
         s = dict(case=case, pages=pages, slots=slots, src=src.to(dev), dst=dst.to(dev),
-                 pairs=list(zip(src.tolist(), dst.tolist())))
+                 pairs=torch.stack([src, dst], 1).to(torch.int32))
         if own:
             from gibbs_b200.ops import RowCopies
             s["copies"] = RowCopies([pages, slots] if slots else [pages])
@@ -368,7 +368,7 @@ def _exact_copy(s):
     """(Moved, not computed.)"""
     for t in s["pages"] + s["slots"]:
         b = _bytes(t)
-        for x, y in (s["pairs"] if t.dim() != 2 or t.dtype != torch.uint8 else [(1, 2)]):
+        for x, y in (s["pairs"].tolist() if t.dim() != 2 or t.dtype != torch.uint8 else [(1, 2)]):
             b[y].copy_(b[x])
     return {"pages": s["pages"], "slots": s["slots"]}
 
