@@ -35,6 +35,8 @@ LIBRARIES = {
     "hybrid": ["errors.cu", "norms.cu", "latent_attention.cu", "latent_attention_tc.cu", "gated_attention.cu", "gated_attention_tc.cu", "gated_attention_tcgen05.cu",
                "sigmoid_attention_tc.cu", "ssm.cu", "selective_scan.cu", "delta_rule.cu", "delta_chunks.cu", "linear_scan.cu", "streams.cu", "moe.cu",
                "moe_tc.cu"],
+    # the 8-bit paged cache: storing, attention, and copies of rows of any cache (forked requests)
+    "kv8": ["errors.cu", "kv8_store.cu", "kv8_attention.cu", "row_copies.cu"],
 }
 
 NVCC_FLAGS = [

@@ -838,3 +838,6 @@ def logprob_info(logits: torch.Tensor, chosen: torch.Tensor, k: int):
                                    _ptr(chosen), _c_int(k), _ptr(prob), _ptr(entropy), _ptr(ids), _ptr(probs),
                                    _stream()))
     return prob, entropy, ids, probs
+
+
+from .row_copies import RowCopies  # noqa: E402  (built from the helpers above)
