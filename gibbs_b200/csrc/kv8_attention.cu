@@ -25,11 +25,12 @@ struct Attn {
   const int* block_table; int bt_stride;
   Step step;
   int parts;                         // CTAs of a cluster
+  int page_shift;                    // log2 of the page size, where that is a power of two
   float scale_log2;                  // scale * log2(e)
   int* status;
 };
 
-constexpr int MAX_PARTS = 8;         // CTAs of a cluster that share a tile's keys
+constexpr int MAX_PARTS = 16;        // CTAs of a cluster that share a tile's keys, at most (8 is the portable limit)
 
 // A tile's request, rows and keys.
 struct Tile {
@@ -258,37 +259,38 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
   join<T, RT, NW>(p, t, kvh, part, parts, m_s, l_s, o_s);
 }
 
-// ---------------------------------------------------------------- bfloat16 on mma.sync
-// Tiles of 16 rows.  K and V stay in 8 bits until they are operands: a lane copies the very bytes of its mma fragments from
-// the pages into shared memory (cp.async, a ring of STAGES chunks per warp, no barrier but the warp's), and turns them into
-// bfloat16 with shifts and masks.  Which entry of a head stands at which place of the contraction is free, as long as q and
-// K agree, and which column of the output belongs to which place of the mma, too: so the places are chosen such that
-//   - of K, lane (g, t) = (lane / 4, lane % 4) holds hd/4 contiguous bytes of key g of a tile of eight keys, four bytes for
-//     each step of 16 entries (bytes 0, 2 in one register, 1, 3 in the other);
-//   - of V, it holds hd/8 contiguous bytes (columns g hd/8 ...) of keys 2t, 2t+1, 2t+8, 2t+9 of 16 keys.
-// The bits s eeee mmm of a number, moved to s 0000eeee mmm0000 of a bfloat16, stand for number * 2^-120 (subnormal numbers
-// included).  The powers of two that are missing go where they are exact and cost nothing: q is multiplied by 2^60 (of q up
-// to 2^67, nothing is lost), the scores by 2^60 and the page's scale, the weights by 2^60 and the page's scale, and the
-// output by 2^60 at the end.
-// The weights are rounded to bfloat16 for the second product (2^-8 of a weight at most, the same as a bfloat16 cache gives);
-// their sum is of the 32-bit weights.
-// Bound by memory from some 4,000 keys a launch's CTA on, below by the chain of trips (metadata, page ids, keys).
+// ---------------------------------------------------------------- bfloat16 rows on mma.sync
+// Tiles of 8 NB rows.  K and V stay in 8 bits until they are operands: a lane copies the very bytes of its mma fragments from
+// the pages into shared memory (cp.async, a ring of STAGES chunks per warp, no barrier but the warp's) and turns two of them at
+// a time into f16, which holds every e4m3 number exactly.  The products are S^T = K Q^T and O^T = V^T P^T: keys (and columns
+// of the output) are the 16 rows of an mma and the few query rows its 8 columns, so that a decoded token of a group of eight
+// heads or fewer wastes little.  Which entry of a head stands at which place of the contraction is free as long as q and K
+// agree, and so is which column of the output has which place: they are chosen such that a lane (g, t) = (lane / 4, lane % 4)
+//   - holds hd/4 contiguous bytes of keys g and g + 8 of sixteen keys, and of q;
+//   - holds hd/8 contiguous bytes (columns g hd/8 ...) of the values of keys 2t, 2t+1, 2t+8, 2t+9.
+// f16 has no room for the scales, so they go elsewhere, where powers of two are exact and cost nothing:
+//   - q's row is multiplied by the power of two that brings its largest magnitude to 2^14 (what is below 2^-28 of that loses
+//     bits; nothing of a bfloat16 above it does), and the scores by its inverse and the page's scale, in 32 bits;
+//   - the page's scale of V goes into the exponent: with x_j = score_j + log2(scale_j) the output is
+//     sum_j 2^(x_j - M) n_j / sum_j 2^(x_j - M) / scale_j, n the stored numbers and M the running maximum of the x.  The weights
+//     w = 2^(x - M + 12) lie below 2^15 and are rounded to f16 (2^-11 of a weight; below 2^-40 of the largest contribution it is
+//     gone, where a 32-bit sum would not see it either); their sum is of the unrounded ones, in 32 bits.
 template <int HD> struct Mma {
-  static constexpr int RT = 16, NW = 4, STAGES = 4;
+  static constexpr int NW = 4, STAGES = 3;
   static constexpr int CK = HD <= 64 ? 32 : 16;                // keys of a chunk
-  static constexpr int NT = CK / 8;                            // tiles of eight keys in it
+  static constexpr int NG = CK / 16;                           // groups of sixteen keys in it: a group lies in one page
   static constexpr int KB = HD / 4, VB = HD / 8;               // bytes of a lane's piece of a key, of a value
   static constexpr int KP = KB % 16 == 0 ? 16 : 8, VP = VB % 16 == 0 ? 16 : VB % 8 == 0 ? 8 : 4;     // bytes of a copy
-  static constexpr int K_STAGE = CK * HD, V_STAGE = CK * HD, META = 2 * NT * 4;
-  static constexpr int STAGE = K_STAGE + V_STAGE + (META + 15) / 16 * 16;
-  static constexpr int JOIN = ((2 * NW + 2) * RT + NW * RT * HD) * 4;
+  static constexpr int K_STAGE = CK * HD, V_STAGE = CK * HD, META = 16;
+  static constexpr int STAGE = K_STAGE + V_STAGE + META;
   static constexpr int RING = NW * STAGES * STAGE;
-  static constexpr int SMEM = RING > JOIN ? RING : JOIN;
+  static constexpr int join(int rt) { return ((2 * NW + 2) * rt + NW * rt * HD) * 4; }
+  static constexpr int smem(int rt) { return RING > join(rt) ? RING : join(rt); }
+  static_assert(2 * NG * 4 <= META, "a scale of K and one of V for each group");
 };
 
 template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t smem, const void* gmem, bool valid) {
-  const int n = valid ? BYTES : 0;                             // 0: the destination is filled with zeros
+__device__ __forceinline__ void cp_async(uint32_t smem, const void* gmem, int n) {             // n = 0: filled with zeros
   if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(n) : "memory");
   else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem), "l"(gmem), "r"(n), "n"(BYTES) : "memory");
 }
@@ -298,31 +300,38 @@ __device__ __forceinline__ void ld_words(uint32_t smem, uint32_t* w) {
   else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(smem));
   else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(smem));
 }
-__device__ __forceinline__ void mma_bf16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
-  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+__device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
+  asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3]) : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8 x 8 matrix of 16-bit entries, two neighbours a lane
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
 }
 __device__ __forceinline__ float ex2(float x) {                // relative error 2^-22; -inf gives 0
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-  const __nv_bfloat162 v = __floats2bfloat162_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&v);
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  uint32_t r;
+  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
 }
-// Bytes 0 and 2 (1 and 3) of a word as two bfloat16, times 2^-120.
-__device__ __forceinline__ uint32_t even_bytes(uint32_t w) { return ((w << 4) & 0x07f007f0u) | ((w << 8) & 0x80008000u); }
-__device__ __forceinline__ uint32_t odd_bytes(uint32_t w) { return ((w >> 4) & 0x07f007f0u) | (w & 0x80008000u); }
+// Bytes 0, 1 (2, 3) of a word as two f16.
+__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
+}
 // 0xff in the bytes that are NaN.
 __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 255u; }
+// log2 and inverse of a power of two (the sign does not matter)
+__device__ __forceinline__ float log2_of(float scale) { return (float)((int)((__float_as_uint(scale) >> 23) & 0xffu) - 127); }
 
-constexpr float TWO_60 = 1152921504606846976.f;
-
-template <int HD>
-__global__ void __launch_bounds__(128, 3) kv8_attention_mma_kernel(const Attn p) {
+template <int HD, int NB>
+__global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
   using C = Mma<HD>;
-  constexpr int RT = C::RT, NW = C::NW, NT = C::NT, CK = C::CK, KW = C::KB / 4, VW = C::VB / 4;
+  constexpr int RT = 8 * NB, NW = C::NW, NG = C::NG, CK = C::CK, KW = C::KB / 4, VW = C::VB / 4;
   extern __shared__ __align__(16) uint8_t smem[];
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
@@ -335,43 +344,48 @@ __global__ void __launch_bounds__(128, 3) kv8_attention_mma_kernel(const Attn p)
   const int* bt = p.block_table + (size_t)t.r * p.bt_stride;
   const int stride = parts * NW, first = part * NW + warp;
 
-  // Lane i looks up the page of tile i of a chunk: id, or -1 where nothing of the tile is visible.
+  // Lane i looks up the page of group i of a chunk: id, or NONE where nothing of the group is visible.
   constexpr int NONE = -1, BAD = -2;
   auto lookup = [&](int c) {
-    const int j = (c_lo + c) * CK + lane * 8;
-    if (lane >= NT || c >= chunks || j >= t.hi || j + 7 < t.lo) return NONE;
-    const int page = bt[j / p.page_size];
+    const int j = (c_lo + c) * CK + lane * 16;
+    if (lane >= NG || c >= chunks || j >= t.hi || j + 15 < t.lo) return NONE;
+    const int page = bt[j >> p.page_shift];
     return page >= 0 && page < p.n_pages ? page : BAD;
   };
   const uint32_t ring = sm100::smem_u32(smem) + (uint32_t)(warp * C::STAGES * C::STAGE);
-  // Requests chunk c into stage `s`; `page` from lookup(c).  A tile without a page is zeros under a scale of 0, which no
+  const uint8_t* k_lane = p.k_pages + (size_t)g * HD + t4 * C::KB;
+  const uint8_t* v_lane = p.v_pages + (size_t)(2 * t4) * HD + g * C::VB;
+  // Requests chunk c into stage `s`; `page` from lookup(c).  A group without a page is zeros under a scale of 0, which no
   // page has: none of its keys is visible.
   auto request = [&](int c, int s, int page) {
     const uint32_t k_at = ring + (uint32_t)(s * C::STAGE), v_at = k_at + C::K_STAGE, m_at = v_at + C::V_STAGE;
-    const int j = (c_lo + c) * CK + lane * 8;
     long long row = -1;
-    if (lane < NT) {
-      const bool valid = page >= 0;
+    if (lane < NG) {
+      const int j = (c_lo + c) * CK + lane * 16;
       if (page == BAD) atomicExch(p.status, STATUS_BAD_PAGE_READ);
-      const size_t ph = valid ? (size_t)page * p.kv_heads + kvh : 0;
-      if (valid) row = ((long long)ph * p.page_size + j % p.page_size) * HD;
-      cp_async<4>(m_at + lane * 4, p.k_scales + ph, valid);
-      cp_async<4>(m_at + (NT + lane) * 4, p.v_scales + ph, valid);
+      const size_t ph = page >= 0 ? (size_t)page * p.kv_heads + kvh : 0;
+      if (page >= 0) row = (long long)((ph << p.page_shift) + (j & (p.page_size - 1))) * HD;
+      cp_async<4>(m_at + lane * 8, p.k_scales + ph, page >= 0 ? 4 : 0);
+      cp_async<4>(m_at + lane * 8 + 4, p.v_scales + ph, page >= 0 ? 4 : 0);
     }
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
+    for (int i = 0; i < NG; ++i) {
       const long long r = __shfl_sync(0xffffffffu, row, i);
-      const uint8_t* kp = p.k_pages + (r < 0 ? 0 : r + g * HD + t4 * C::KB);
+      const bool valid = r >= 0;
+      const uint8_t* kp = k_lane + (valid ? r : 0);            // (zero bytes are read of a group without a page, from page 0)
+      const uint8_t* vp = v_lane + (valid ? r : 0);
 #pragma unroll
-      for (int x = 0; x < C::KB / C::KP; ++x)
-        cp_async<C::KP>(k_at + (uint32_t)(((i * (C::KB / C::KP) + x) * 32 + lane) * C::KP), kp + x * C::KP, r >= 0);
-      // keys 2t, 2t + 1 of the tile
-      const uint8_t* vp = p.v_pages + (r < 0 ? 0 : r + 2 * t4 * HD + g * C::VB);
+      for (int y = 0; y < 2; ++y)                              // keys g, g + 8
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
+        for (int x = 0; x < C::KB / C::KP; ++x)
+          cp_async<C::KP>(k_at + (uint32_t)((((2 * i + y) * (C::KB / C::KP) + x) * 32 + lane) * C::KP), kp + y * 8 * HD + x * C::KP,
+                          valid ? C::KP : 0);
+#pragma unroll
+      for (int y = 0; y < 4; ++y)                              // keys 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
         for (int x = 0; x < C::VB / C::VP; ++x)
-          cp_async<C::VP>(v_at + (uint32_t)((((2 * i + y) * (C::VB / C::VP) + x) * 32 + lane) * C::VP), vp + (r < 0 ? 0 : y * HD + x * C::VP), r >= 0);
+          cp_async<C::VP>(v_at + (uint32_t)((((4 * i + y) * (C::VB / C::VP) + x) * 32 + lane) * C::VP),
+                          vp + ((y & 1) + 4 * (y & 2)) * HD + x * C::VP, valid ? C::VP : 0);
     }
   };
   int pages[C::STAGES];
@@ -385,19 +399,18 @@ __global__ void __launch_bounds__(128, 3) kv8_attention_mma_kernel(const Attn p)
   }
   int page_next = pages[C::STAGES - 1];
 
-  // q: rows g and g + 8, entries t4 * KB ... + KB, times 2^60
-  uint32_t qa[HD / 16][4];
-  int rpos[2];
-  const bool upper = t.rows > 8;
+  // q: row g of each block, entries t4 * KB ... + KB, under its power of two.  In the lane's columns of S^T and O^T stand rows
+  // 2t and 2t + 1 of each block.
+  uint32_t qb[NB][HD / 16][2];
+  int rpos[NB][2];
+  float factor[NB][2];                                         // scale * log2(e) / the row's power of two
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int row = g + 8 * i;
-    rpos[i] = -1;                                              // (a row that does not exist sees nothing)
+  for (int b = 0; b < NB; ++b) {
+    const int row = 8 * b + g;
     uint32_t w[HD / 8];
 #pragma unroll
     for (int x = 0; x < HD / 8; ++x) w[x] = 0u;
     if (row < t.rows) {
-      rpos[i] = t.pos(row);
       const int tok = (t.row0 + row) / t.group, h = (t.row0 + row) - tok * t.group;
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(p.q) + (size_t)(t.qstart + tok) * p.ldq +
                                                         (size_t)(kvh * t.group + h) * HD + t4 * C::KB);
@@ -406,26 +419,39 @@ __global__ void __launch_bounds__(128, 3) kv8_attention_mma_kernel(const Attn p)
         const uint4 u = src[x];
         w[4 * x] = u.x; w[4 * x + 1] = u.y; w[4 * x + 2] = u.z; w[4 * x + 3] = u.w;
       }
-      const __nv_bfloat162 up = __floats2bfloat162_rn(TWO_60, TWO_60);
-#pragma unroll
-      for (int x = 0; x < HD / 8; ++x) {
-        const __nv_bfloat162 v = __hmul2(*reinterpret_cast<__nv_bfloat162*>(&w[x]), up);
-        w[x] = *reinterpret_cast<const uint32_t*>(&v);
-      }
     }
+    uint32_t top = 0u;                                         // largest magnitude: bits of a bfloat16 compare like a number's
 #pragma unroll
-    for (int kk = 0; kk < HD / 16; ++kk) {
-      qa[kk][i] = __byte_perm(w[2 * kk], w[2 * kk + 1], 0x5410);       // entries 0, 2 of four
-      qa[kk][2 + i] = __byte_perm(w[2 * kk], w[2 * kk + 1], 0x7632);   // entries 1, 3
+    for (int x = 0; x < HD / 8; ++x) top = max(top, max(w[x] & 0x7fffu, (w[x] >> 16) & 0x7fffu));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+    const int e = min(127, max((int)(top >> 7) - 127, -112));  // (a row of zeros, or one that is not finite, under any power)
+    const float up = pow2(min(14 - e, 126)), back = p.scale_log2 * pow2(max(e - 14, -126));
+#pragma unroll
+    for (int kk = 0; kk < HD / 16; ++kk)
+#pragma unroll
+      for (int y = 0; y < 2; ++y) {
+        const uint32_t v = w[2 * kk + y];
+        qb[b][kk][y] = pack_f16(__uint_as_float(v << 16) * up, __uint_as_float(v & 0xffff0000u) * up);
+      }
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+      factor[b][r] = __shfl_sync(0xffffffffu, back, (2 * t4 + r) * 4);
+      const int mine = 8 * b + 2 * t4 + r;
+      rpos[b][r] = mine < t.rows ? t.pos(mine) : -1;           // (a row that does not exist sees nothing)
     }
   }
 
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-  float o[HD / 8][4];
+  float m[NB][2], l[NB][2], o[NB][HD / 16][4];
 #pragma unroll
-  for (int n = 0; n < HD / 8; ++n)
+  for (int b = 0; b < NB; ++b) {
+    m[b][0] = m[b][1] = -INFINITY;
+    l[b][0] = l[b][1] = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) o[n][i] = 0.f;
+    for (int n = 0; n < HD / 16; ++n)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) o[b][n][i] = 0.f;
+  }
   const int pos_first = t.pos(0), pos_last = t.pos(t.rows - 1);
 
   int stage = 0;
@@ -440,103 +466,120 @@ __global__ void __launch_bounds__(128, 3) kv8_attention_mma_kernel(const Attn p)
     }
     const uint32_t k_at = ring + (uint32_t)(stage * C::STAGE), v_at = k_at + C::K_STAGE, m_at = v_at + C::V_STAGE;
     stage = stage == C::STAGES - 1 ? 0 : stage + 1;
-    float s[NT][4], vs[NT];
-    float top[2] = {-INFINITY, -INFINITY};
+    float s[NB][NG][4], ks[NG], vs[NG];
     bool careful = false;                                      // some page of the chunk has NaN among its values
 #pragma unroll
-    for (int i = 0; i < NT; ++i) {
-      float ks;
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(ks) : "r"(m_at + i * 4));
-      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(vs[i]) : "r"(m_at + (NT + i) * 4));
+    for (int i = 0; i < NG; ++i) {
+      uint32_t sc[2];
+      ld_words<2>(m_at + i * 8, sc);
+      ks[i] = __uint_as_float(sc[0]);
+      vs[i] = __uint_as_float(sc[1]);
       careful |= vs[i] < 0.f;
-      vs[i] = fabsf(vs[i]) * TWO_60;
-      uint32_t w[KW];
+      uint32_t w[2][KW];
 #pragma unroll
-      for (int x = 0; x < C::KB / C::KP; ++x)
-        ld_words<C::KP / 4>(k_at + (uint32_t)(((i * (C::KB / C::KP) + x) * 32 + lane) * C::KP), w + x * (C::KP / 4));
+      for (int y = 0; y < 2; ++y)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] = 0.f;
+        for (int x = 0; x < C::KB / C::KP; ++x)
+          ld_words<C::KP / 4>(k_at + (uint32_t)((((2 * i + y) * (C::KB / C::KP) + x) * 32 + lane) * C::KP), w[y] + x * (C::KP / 4));
 #pragma unroll
-      for (int kk = 0; kk < HD / 16; ++kk) mma_bf16(s[i], qa[kk], even_bytes(w[kk]), odd_bytes(w[kk]));
-      const float factor = fabsf(ks) * (TWO_60 * p.scale_log2);
+      for (int b = 0; b < NB; ++b)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) s[i][e] *= factor;
-      if (ks < 0.f) {
-        // keys with a NaN: lanes 4k .. 4k + 3 hold key k; this lane's columns are keys 2t, 2t + 1
-        uint32_t any = 0u;
+        for (int e = 0; e < 4; ++e) s[b][i][e] = 0.f;
 #pragma unroll
-        for (int kk = 0; kk < KW; ++kk) any |= nan_bytes(w[kk]);
-        const uint32_t keys = __ballot_sync(0xffffffffu, any != 0u) >> (8 * t4);
-        if (keys & 0xfu) s[i][0] = s[i][2] = __int_as_float(0x7fffffff);
-        if (keys & 0xf0u) s[i][1] = s[i][3] = __int_as_float(0x7fffffff);
+      for (int kk = 0; kk < HD / 16; ++kk) {
+        uint32_t a[4];
+        to_f16(w[0][kk], a[0], a[2]);
+        to_f16(w[1][kk], a[1], a[3]);
+#pragma unroll
+        for (int b = 0; b < NB; ++b) mma_f16(s[b][i], a, qb[b][kk][0], qb[b][kk][1]);
       }
-      const int j0 = (c_lo + c) * CK + 8 * i;
-      const bool full = ks != 0.f && j0 + 7 <= pos_first && (p.window <= 0 || j0 + p.window > pos_last);
-      if (!full) {
+      // x = score + log2(scale of V), -inf where a row does not see the key
+      const int j0 = (c_lo + c) * CK + 16 * i;
+      const bool full = ks[i] != 0.f && j0 + 15 <= pos_first && (p.window <= 0 || j0 + p.window > pos_last);
+      const float lv = log2_of(vs[i]), kf = fabsf(ks[i]);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int j = j0 + 2 * t4 + (e & 1), pos = rpos[e >> 1];
-          const bool seen = ks != 0.f && j <= pos && (p.window <= 0 || j + p.window > pos);
-          s[i][e] = seen ? s[i][e] : -INFINITY;
+      for (int b = 0; b < NB; ++b) {
+        const float f0 = factor[b][0] * kf, f1 = factor[b][1] * kf;
+        s[b][i][0] = fmaf(s[b][i][0], f0, lv);
+        s[b][i][1] = fmaf(s[b][i][1], f1, lv);
+        s[b][i][2] = fmaf(s[b][i][2], f0, lv);
+        s[b][i][3] = fmaf(s[b][i][3], f1, lv);
+        if (!full) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int j = j0 + g + 8 * (e >> 1), pos = rpos[b][e & 1];
+            const bool seen = ks[i] != 0.f && j <= pos && (p.window <= 0 || j + p.window > pos);
+            s[b][i][e] = seen ? s[b][i][e] : -INFINITY;
+          }
         }
       }
-      top[0] = fmaxf(top[0], fmaxf(s[i][0], s[i][1]));
-      if (upper) top[1] = fmaxf(top[1], fmaxf(s[i][2], s[i][3]));
     }
-    // The maximum in use follows a row's only when it would fall behind by more than 2^8: weights stay below 256, and most
-    // chunks leave the output as it is.
-    float corr[2] = {1.f, 1.f}, use[2];
+    // The maximum in use follows a row's only when it would fall behind by more than 2^3: a weight stays below 2^15.
 #pragma unroll
-    for (int r = 0; r < 2; ++r) {
-      if (r == 0 || upper) {
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 1));
-        top[r] = fmaxf(top[r], __shfl_xor_sync(0xffffffffu, top[r], 2));
-        if (top[r] > m[r] + 8.f || (m[r] == -INFINITY && top[r] > -INFINITY)) {
-          corr[r] = ex2(m[r] - top[r]);                        // 0 when nothing was seen before
-          m[r] = top[r];
-          l[r] *= corr[r];
+    for (int b = 0; b < NB; ++b) {
+      float corr[2];
+      bool grow = false;
+#pragma unroll
+      for (int r = 0; r < 2; ++r) {
+        float top = fmaxf(s[b][0][r], s[b][0][r + 2]);
+#pragma unroll
+        for (int i = 1; i < NG; ++i) top = fmaxf(top, fmaxf(s[b][i][r], s[b][i][r + 2]));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+        corr[r] = 1.f;
+        if (top > m[b][r] + 3.f || (m[b][r] == -INFINITY && top > -INFINITY)) {
+          corr[r] = ex2(m[b][r] - top);                        // 0 when nothing was seen before
+          m[b][r] = top;
+          l[b][r] *= corr[r];
+          grow = true;
         }
       }
-      use[r] = m[r] == -INFINITY ? 0.f : m[r];
-    }
-    if (corr[0] != 1.f || corr[1] != 1.f) {
+      if (grow) {
 #pragma unroll
-      for (int n = 0; n < HD / 8; ++n) {
-        o[n][0] *= corr[0]; o[n][1] *= corr[0];
-        o[n][2] *= corr[1]; o[n][3] *= corr[1];
+        for (int n = 0; n < HD / 16; ++n) {
+          o[b][n][0] *= corr[0]; o[b][n][1] *= corr[1];
+          o[b][n][2] *= corr[0]; o[b][n][3] *= corr[1];
+        }
       }
     }
 #pragma unroll
-    for (int x = 0; x < NT / 2; ++x) {                         // 16 keys
-      uint32_t a[4], see[4];
+    for (int i = 0; i < NG; ++i) {
+      uint32_t pb[NB][2];
+      const float inv = inverse(vs[i]);
 #pragma unroll
-      for (int y = 0; y < 2; ++y) {
-        float* sv = s[2 * x + y];
-        const float e0 = ex2(sv[0] - use[0]), e1 = ex2(sv[1] - use[0]);
-        l[0] += e0 + e1;
-        a[2 * y] = pack_bf16(e0 * vs[2 * x + y], e1 * vs[2 * x + y]);
-        a[2 * y + 1] = 0u;
-        if (upper) {
-          const float e2 = ex2(sv[2] - use[1]), e3 = ex2(sv[3] - use[1]);
-          l[1] += e2 + e3;
-          a[2 * y + 1] = pack_bf16(e2 * vs[2 * x + y], e3 * vs[2 * x + y]);
-        }
+      for (int b = 0; b < NB; ++b) {
+        const float u0 = (m[b][0] == -INFINITY ? 0.f : m[b][0]) - 12.f, u1 = (m[b][1] == -INFINITY ? 0.f : m[b][1]) - 12.f;
+        const float e0 = ex2(s[b][i][0] - u0), e1 = ex2(s[b][i][1] - u1), e2 = ex2(s[b][i][2] - u0), e3 = ex2(s[b][i][3] - u1);
+        l[b][0] = fmaf(e0 + e2, inv, l[b][0]);
+        l[b][1] = fmaf(e1 + e3, inv, l[b][1]);
+        pb[b][0] = transposed(pack_f16(e0, e1));               // keys 0..7 of the group, then 8..15
+        pb[b][1] = transposed(pack_f16(e2, e3));
       }
       uint32_t v[4][VW];
 #pragma unroll
-      for (int y = 0; y < 4; ++y)                              // keys 2t, 2t + 1 of the first tile, then of the second
+      for (int y = 0; y < 4; ++y)
 #pragma unroll
-        for (int z = 0; z < C::VB / C::VP; ++z)
-          ld_words<C::VP / 4>(v_at + (uint32_t)((((4 * x + y) * (C::VB / C::VP) + z) * 32 + lane) * C::VP), v[y] + z * (C::VP / 4));
+        for (int x = 0; x < C::VB / C::VP; ++x)
+          ld_words<C::VP / 4>(v_at + (uint32_t)((((4 * i + y) * (C::VB / C::VP) + x) * 32 + lane) * C::VP), v[y] + x * (C::VP / 4));
+      const int j0 = (c_lo + c) * CK + 16 * i;
+      if (j0 + 16 > t.hi) {                                    // rows behind the context hold anything: 0 * NaN is not 0
+#pragma unroll
+        for (int y = 0; y < 4; ++y)
+          if (j0 + 2 * t4 + (y & 1) + 4 * (y & 2) >= t.hi) {
+#pragma unroll
+            for (int w = 0; w < VW; ++w) v[y][w] = 0u;
+          }
+      }
       if (careful) {
-        // A NaN reaches the rows that see its key and no other: the numbers go in as 0, and rows (1: sees) times columns
-        // (1: NaN) tell where the output is NaN.
+        // A NaN reaches the rows that see its key and no other: the numbers go in as 0, and (columns of a key that are NaN)
+        // times (rows that see the key) tells where the output is NaN.
+        uint32_t see[NB][2];
 #pragma unroll
-        for (int y = 0; y < 2; ++y) {
-          const float* sv = s[2 * x + y];
-          see[2 * y] = pack_bf16(sv[0] == -INFINITY ? 0.f : 1.f, sv[1] == -INFINITY ? 0.f : 1.f);
-          see[2 * y + 1] = pack_bf16(sv[2] == -INFINITY ? 0.f : 1.f, sv[3] == -INFINITY ? 0.f : 1.f);
-        }
+        for (int b = 0; b < NB; ++b)
+#pragma unroll
+          for (int y = 0; y < 2; ++y)
+            see[b][y] = transposed(pack_f16(s[b][i][2 * y] == -INFINITY ? 0.f : 1.f, s[b][i][2 * y + 1] == -INFINITY ? 0.f : 1.f));
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t bad[4];
@@ -546,25 +589,34 @@ __global__ void __launch_bounds__(128, 3) kv8_attention_mma_kernel(const Attn p)
             v[y][w] &= ~bad[y];
           }
 #pragma unroll
-          for (int z = 0; z < 4; ++z) {
-            const uint32_t lo = __byte_perm(bad[0], bad[1], z < 2 ? 0x5410 : 0x7632), hi = __byte_perm(bad[2], bad[3], z < 2 ? 0x5410 : 0x7632);
-            float n[4] = {0.f, 0.f, 0.f, 0.f};
-            mma_bf16(n, see, (z & 1 ? lo : lo << 8) & 0x3f003f00u, (z & 1 ? hi : hi << 8) & 0x3f003f00u);
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t lo = __byte_perm(bad[0], bad[1], h ? 0x7362 : 0x5140), hi = __byte_perm(bad[2], bad[3], h ? 0x7362 : 0x5140);
+            uint32_t a[4];                                     // 1 (f16) where a number is NaN
+            a[0] = __byte_perm(lo, 0u, 0x1404) & 0x3c003c00u;
+            a[1] = __byte_perm(lo, 0u, 0x3424) & 0x3c003c00u;
+            a[2] = __byte_perm(hi, 0u, 0x1404) & 0x3c003c00u;
+            a[3] = __byte_perm(hi, 0u, 0x3424) & 0x3c003c00u;
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n[e] > 0.f) o[4 * w + z][e] = __int_as_float(0x7fffffff);
+            for (int b = 0; b < NB; ++b) {
+              float n[4] = {0.f, 0.f, 0.f, 0.f};
+              mma_f16(n, a, see[b][0], see[b][1]);
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n[e] > 0.f) o[b][2 * w + h][e] = __int_as_float(0x7fffffff);
+            }
           }
         }
       }
 #pragma unroll
-      for (int w = 0; w < VW; ++w) {
-        const uint32_t l0 = __byte_perm(v[0][w], v[1][w], 0x5410), l1 = __byte_perm(v[0][w], v[1][w], 0x7632);
-        const uint32_t h0 = __byte_perm(v[2][w], v[3][w], 0x5410), h1 = __byte_perm(v[2][w], v[3][w], 0x7632);
-        mma_bf16(o[4 * w], a, even_bytes(l0), even_bytes(h0));
-        mma_bf16(o[4 * w + 1], a, odd_bytes(l0), odd_bytes(h0));
-        mma_bf16(o[4 * w + 2], a, even_bytes(l1), even_bytes(h1));
-        mma_bf16(o[4 * w + 3], a, odd_bytes(l1), odd_bytes(h1));
-      }
+      for (int w = 0; w < VW; ++w)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t a[4];
+          to_f16(__byte_perm(v[0][w], v[1][w], h ? 0x7362 : 0x5140), a[0], a[1]);
+          to_f16(__byte_perm(v[2][w], v[3][w], h ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+          for (int b = 0; b < NB; ++b) mma_f16(o[b][2 * w + h], a, pb[b][0], pb[b][1]);
+        }
     }
   }
   asm volatile("cp.async.wait_group 0;" ::: "memory");
@@ -573,24 +625,22 @@ __global__ void __launch_bounds__(128, 3) kv8_attention_mma_kernel(const Attn p)
   float* l_s = m_s + (NW + 2) * RT;                            // [NW][RT]
   float* o_s = l_s + NW * RT;                                  // [NW][RT][HD]
 #pragma unroll
-  for (int r = 0; r < 2; ++r) {
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 1);
-    l[r] += __shfl_xor_sync(0xffffffffu, l[r], 2);
-    const int row = g + 8 * r;
-    if (row >= t.rows) continue;
-    if (t4 == 0) {
-      m_s[warp * RT + row] = m[r];
-      l_s[warp * RT + row] = l[r];
+  for (int b = 0; b < NB; ++b)
+#pragma unroll
+    for (int r = 0; r < 2; ++r) {
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2) l[b][r] += __shfl_xor_sync(0xffffffffu, l[b][r], x);
+      const int row = 8 * b + 2 * t4 + r;
+      if (row >= t.rows) continue;
+      if (g == 0) {
+        m_s[warp * RT + row] = m[b][r];
+        l_s[warp * RT + row] = l[b][r];
+      }
+      float* at = o_s + ((size_t)warp * RT + row) * HD + g * C::VB;
+#pragma unroll
+      for (int n = 0; n < HD / 16; n += 2)
+        *reinterpret_cast<float4*>(at + 2 * n) = make_float4(o[b][n][r], o[b][n][r + 2], o[b][n + 1][r], o[b][n + 1][r + 2]);
     }
-    float* at = o_s + ((size_t)warp * RT + row) * HD;
-#pragma unroll
-    for (int n = 0; n < HD / 8; n += 4)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-        *reinterpret_cast<float4*>(at + (2 * t4 + e) * C::VB + n) =
-            make_float4(o[n][2 * r + e] * TWO_60, o[n + 1][2 * r + e] * TWO_60, o[n + 2][2 * r + e] * TWO_60,
-                        o[n + 3][2 * r + e] * TWO_60);
-  }
   join<bf16, RT, NW>(p, t, kvh, part, parts, m_s, l_s, o_s);
 }
 
@@ -634,6 +684,11 @@ template <typename T, int NP>
 int launch_any(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
   constexpr int RT = 4, NW = 4;
   const size_t smem = (size_t)(RT * p.hd + (2 * NW + 2) * RT + NW * RT * p.hd) * 4 + NW * 32 * (16 + 8);
+  static bool attr_set = false;
+  if (!attr_set) {
+    GB_CUDA(cudaFuncSetAttribute(kv8_attention_any_kernel<T, NP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    attr_set = true;
+  }
   return launch_parts(kv8_attention_any_kernel<T, NP>, p, key_parts(tiles * p.kv_heads, 148 * 4, (keys + 31) / 32, NW), tiles, 32 * NW,
                       smem, stream);
 }
@@ -647,16 +702,27 @@ int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t st
   }
 }
 
-template <int HD>
+template <int HD, int NB>
 int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
   using C = Mma<HD>;
+  constexpr int SMEM = C::smem(8 * NB), SLOTS = 227 * 1024 / (SMEM + 1024) < 4 ? 227 * 1024 / (SMEM + 1024) : 4;
   static bool attr_set = false;
   if (!attr_set) {
-    GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM));
+    GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set = true;
   }
-  return launch_parts(kv8_attention_mma_kernel<HD>, p, key_parts(tiles * p.kv_heads, 148 * 3, (keys + C::CK - 1) / C::CK, C::NW), tiles,
-                      32 * C::NW, C::SMEM, stream);
+  return launch_parts(kv8_attention_mma_kernel<HD, NB>, p, key_parts(tiles * p.kv_heads, 148 * SLOTS, (keys + C::CK - 1) / C::CK, C::NW),
+                      tiles, 32 * C::NW, SMEM, stream);
+}
+template <int NB>
+int dispatch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
+  switch (p.hd) {
+    case 32: return launch_mma<32, NB>(p, tiles, keys, stream);
+    case 64: return launch_mma<64, NB>(p, tiles, keys, stream);
+    case 96: return launch_mma<96, NB>(p, tiles, keys, stream);
+    default: return launch_mma<128, NB>(p, tiles, keys, stream);
+  }
 }
 
 }  // namespace
@@ -690,18 +756,21 @@ GB_OP(gb_op_kv8_attention) {
             p.heads, p.kv_heads, p.hd, p.page_size);
   if (dtype != GB_F32 && dtype != GB_BF16) GB_FAIL(GB_ERR_ARG, "kv8_attention: q and out are float32 or bfloat16");
   const int group = p.heads / p.kv_heads;
-  const bool mma = dtype == GB_BF16 && (p.hd == 32 || p.hd == 64 || p.hd == 96 || p.hd == 128) && p.page_size % 8 == 0 &&
-                   p.ldq % 8 == 0 && ((uintptr_t)p.q & 15) == 0;
+  p.page_shift = 0;
+  while ((1 << p.page_shift) < p.page_size) ++p.page_shift;
+  const bool mma = dtype == GB_BF16 && (p.hd == 32 || p.hd == 64 || p.hd == 96 || p.hd == 128) && p.page_size >= 16 &&
+                   (1 << p.page_shift) == p.page_size && p.ldq % 8 == 0 && ((uintptr_t)p.q & 15) == 0;
+  // rows of a tile: with 8, a step of single tokens in groups of eight heads or fewer; with 16, half as many passes over the keys
+  const bool small = (long long)p.step.max_q * group <= 8;
   // upper bound of the tiles: sum_r ceil(q_len_r * group / rt)
-  const int rt = mma ? 16 : 4;
+  const int rt = !mma ? 4 : small ? 8 : 16;
   const long long tiles = p.step.one_each ? (long long)p.step.n_requests * ((group + rt - 1) / rt)
                                           : (long long)p.step.n_tokens * group / rt + p.step.n_requests;
   if (tiles * p.kv_heads > 0x7fffffff / MAX_PARTS) GB_FAIL(GB_ERR_ARG, "kv8_attention: %lld tiles in one launch", tiles);
   const long long keys = p.window > 0 && p.window + rt < p.step.max_ctx ? p.window + rt : p.step.max_ctx;
   int rc;
   if (mma)
-    rc = p.hd == 32 ? launch_mma<32>(p, tiles, keys, ctx->stream) : p.hd == 64 ? launch_mma<64>(p, tiles, keys, ctx->stream)
-         : p.hd == 96 ? launch_mma<96>(p, tiles, keys, ctx->stream) : launch_mma<128>(p, tiles, keys, ctx->stream);
+    rc = small ? dispatch_mma<1>(p, tiles, keys, ctx->stream) : dispatch_mma<2>(p, tiles, keys, ctx->stream);
   else
     rc = dtype == GB_F32 ? dispatch_any<float>(p, tiles, keys, ctx->stream) : dispatch_any<bf16>(p, tiles, keys, ctx->stream);
   if (rc != GB_OK) return rc;

@@ -74,10 +74,12 @@ class PlainPages:
         self.written[page, first:first + m] = True
 
 
-def attention(q, keys, values, scale, window, pos):
+def attention(q, keys, values, scale, window, pos, page_scales=None):
     """softmax(scale q K^T) V of rows q [n, group, hd] at positions pos [n] over keys, values [L, hd] (position j in row j), all
-    64-bit; also sum p |v| per entry and the largest sum |q||k| scale of a visible key per row."""
+    64-bit; also sum p |v| per entry, the largest sum |q||k| scale of a visible key per row and, with ``page_scales`` [L] (of
+    the values), the number of visible keys times the largest p * page scale per row."""
     j = torch.arange(keys.shape[0])
+    most = torch.zeros(q.shape, dtype=torch.float64)
     out, weight, spread = (torch.zeros(q.shape, dtype=torch.float64) for _ in range(3))
     for i in range(q.shape[0]):
         seen = (j <= pos[i]) & ((j > pos[i] - window) if window else (j >= 0))
@@ -87,4 +89,6 @@ def attention(q, keys, values, scale, window, pos):
         out[i] = p @ v
         weight[i] = p @ v.abs()
         spread[i] = ((q[i].abs() @ k.abs().T) * scale).amax(-1, keepdim=True)
-    return out, weight, spread
+        if page_scales is not None:
+            most[i] = (p.nan_to_num() * page_scales[seen]).amax(-1, keepdim=True) * int(seen.sum())
+    return (out, weight, spread) if page_scales is None else (out, weight, spread, most)

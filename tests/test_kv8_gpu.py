@@ -324,14 +324,16 @@ def attention_case(dtype, heads, kv_heads, hd, page, window, portions, behind, s
     assert int(step.status.item()) == 0
     keys, values = (t.double().cpu() for t in pages.dequantized())
     q = wide[:n, :heads * hd].double().view(n, kv_heads, group, hd)
-    want, weight, spread = (torch.zeros(n, kv_heads, group, hd, dtype=torch.float64) for _ in range(3))
+    want, weight, spread, largest = (torch.zeros(n, kv_heads, group, hd, dtype=torch.float64) for _ in range(4))
+    scales = pages.v_scales.abs().double().cpu()
     row = 0
     for r, (p, b) in enumerate(zip(portions, behind)):
         ids = bt[r, :-(-(p + b) // page)].long().clamp(min=0)
         for h in range(kv_heads):
             k, v = (t[ids, h].reshape(-1, hd) for t in (keys, values))
             s = slice(row, row + p)
-            want[s, h], weight[s, h], spread[s, h] = plain.attention(q[s, h], k, v, scale, window, torch.arange(b, b + p))
+            want[s, h], weight[s, h], spread[s, h], largest[s, h] = plain.attention(
+                q[s, h], k, v, scale, window, torch.arange(b, b + p), scales[ids, h].repeat_interleave(page))
         row += p
     got = out.cpu()
     assert bool((got[n:] == 7.0).all())
@@ -341,7 +343,11 @@ def attention_case(dtype, heads, kv_heads, hd, page, window, portions, behind, s
     soft = 2 * (hd + 8) * 2.0 ** -23 * spread + (most + 64) * 2.0 ** -23
     tol = soft * weight + (2.0 ** -18 * weight)
     if dt == torch.bfloat16:
-        tol = tol + 2.0 ** -8 * weight + 2.0 ** -8 * want.abs()          # weights in bfloat16, and the output's own rounding
+        tol = tol + 2.0 ** -8 * weight + 2.0 ** -8 * want.abs()          # weights in 16 bits, and the output's own rounding
+        # Weights p_j s_j (s_j: the page's scale) are held in f16 as w = p_j s_j 2^12 / u, u the largest that the running maximum
+        # has seen (or up to 2^3 below it), so u <= max_j p_j s_j.  An f16 of w is off by 2^-25 at most where it is subnormal:
+        # an output by sum_j 2^-25 2^-12 u |n_j| <= 2^-37 * 448 * (number of keys) * max_j p_j s_j.
+        tol = tol + 2.0 ** -37 * 448 * largest
     return got[:n].double().view(want.shape), want, tol
 
 
