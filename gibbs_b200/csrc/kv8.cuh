@@ -10,6 +10,8 @@
 // What is not finite, or above 448 * 2^50 (5e17), is stored as NaN, does not count for the scale, and makes the scale's sign
 // NEGATIVE: kernels take the careful way through such a page, and pay nothing for NaN anywhere else.
 #pragma once
+#include <cuda.h>
+
 #include "common.cuh"
 #include "gb_plan_op.h"
 
@@ -122,6 +124,21 @@ __device__ __forceinline__ int find_piece(int index, int n_requests, bool last_f
     index -= __shfl_sync(0xffffffffu, upto, 31);
   }
   return -1;
+}
+
+// The driver's cuTensorMapEncodeTiled (null where there is none).
+typedef CUresult (*TensorMapFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline TensorMapFn tensor_map_fn() {
+  static const TensorMapFn fn = [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool found = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) == cudaSuccess &&
+                       q == cudaDriverEntryPointSuccess;
+    return found ? (TensorMapFn)p : (TensorMapFn) nullptr;
+  }();
+  return fn;
 }
 
 }  // namespace kv8

@@ -30,6 +30,7 @@ struct Attn {
   int* status;
 };
 
+constexpr int STATUS_TIMEOUT = 40;   // a bounded wait ran out
 constexpr int MAX_PARTS = 16;        // CTAs of a cluster that share a tile's keys, at most (8 is the portable limit)
 
 // A tile's request, rows and keys.
@@ -260,14 +261,13 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
 }
 
 // ---------------------------------------------------------------- bfloat16 rows on mma.sync
-// Tiles of 8 NB rows.  K and V stay in 8 bits until they are operands: a lane copies the very bytes of its mma fragments from
-// the pages into shared memory (cp.async, a ring of STAGES chunks per warp, no barrier but the warp's) and turns two of them at
-// a time into f16, which holds every e4m3 number exactly.  The products are S^T = K Q^T and O^T = V^T P^T: keys (and columns
+// Tiles of 8 NB rows.  K and V stay in 8 bits until they are operands: a lane reads the bytes of its mma fragments and turns two
+// of them at a time into f16, which holds every e4m3 number exactly.  The products are S^T = K Q^T and O^T = V^T P^T: keys (and columns
 // of the output) are the 16 rows of an mma and the few query rows its 8 columns, so that a decoded token of a group of eight
 // heads or fewer wastes little.  Which entry of a head stands at which place of the contraction is free as long as q and K
 // agree, and so is which column of the output has which place: they are chosen such that a lane (g, t) = (lane / 4, lane % 4)
-//   - holds hd/4 contiguous bytes of keys g and g + 8 of sixteen keys, and of q;
-//   - holds hd/8 contiguous bytes (columns g hd/8 ...) of the values of keys 2t, 2t+1, 2t+8, 2t+9.
+//   - holds hd/4 contiguous bytes of the keys in places g and g + 8 of sixteen, and of q;
+//   - holds hd/8 contiguous bytes (columns g hd/8 ...) of the values in places 2t, 2t+1, 2t+8, 2t+9.
 // f16 has no room for the scales, so they go elsewhere, where powers of two are exact and cost nothing:
 //   - q's row is multiplied by the power of two that brings its largest magnitude to 2^14 (what is below 2^-28 of that loses
 //     bits; nothing of a bfloat16 above it does), and the scores by its inverse and the page's scale, in 32 bits;
@@ -275,30 +275,44 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
 //     sum_j 2^(x_j - M) n_j / sum_j 2^(x_j - M) / scale_j, n the stored numbers and M the running maximum of the x.  The weights
 //     w = 2^(x - M + 12) lie below 2^15 and are rounded to f16 (2^-11 of a weight; below 2^-40 of the largest contribution it is
 //     gone, where a 32-bit sum would not see it either); their sum is of the unrounded ones, in 32 bits.
+// K and V come by TMA, sixteen keys (a group, which lies in one page) a copy, into a ring of SLOTS slots per warp: no barrier but
+// the warp's own, and a copy costs an instruction instead of one for every lane and piece.  The rows are swizzled (128-byte
+// rows by the 16-byte piece XOR row, 64-byte rows by piece XOR row / 2) and the keys of a group take the places pi(0..15) of the
+// products: with these every fragment is read without a bank conflict.
 template <int HD> struct Mma {
-  static constexpr int NW = 4, STAGES = 3;
-  static constexpr int CK = HD <= 64 ? 32 : 16;                // keys of a chunk
-  static constexpr int NG = CK / 16;                           // groups of sixteen keys in it: a group lies in one page
+  static constexpr int NW = 4;
+  static constexpr int NG = 2;                                 // groups of a slot, taken together
+  static constexpr int SLOTS = HD <= 64 ? 3 : 2;
+  static constexpr int CTAS = HD <= 64 ? 4 : 3;                // on an SM: by shared memory, and registers capped to that
+  static constexpr int CK = 16 * NG;                           // keys of a chunk
   static constexpr int KB = HD / 4, VB = HD / 8;               // bytes of a lane's piece of a key, of a value
-  static constexpr int KP = KB % 16 == 0 ? 16 : 8, VP = VB % 16 == 0 ? 16 : VB % 8 == 0 ? 8 : 4;     // bytes of a copy
-  static constexpr int K_STAGE = CK * HD, V_STAGE = CK * HD, META = 16;
-  static constexpr int STAGE = K_STAGE + V_STAGE + META;
-  static constexpr int RING = NW * STAGES * STAGE;
+  static constexpr int GROUP = 16 * HD;                        // bytes of a group's keys
+  static constexpr int SLOT = 2 * NG * GROUP;
+  static constexpr int RING = NW * SLOTS * SLOT;
   static constexpr int join(int rt) { return ((2 * NW + 2) * rt + NW * rt * HD) * 4; }
-  static constexpr int smem(int rt) { return RING > join(rt) ? RING : join(rt); }
-  static_assert(2 * NG * 4 <= META, "a scale of K and one of V for each group");
+  static constexpr int smem(int rt) { return (RING > join(rt) ? RING : join(rt)) + 1024; }
 };
 
-template <int BYTES>
-__device__ __forceinline__ void cp_async(uint32_t smem, const void* gmem, int n) {             // n = 0: filled with zeros
-  if constexpr (BYTES == 16) asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(n) : "memory");
-  else asm volatile("cp.async.ca.shared.global [%0], [%1], %3, %2;" ::"r"(smem), "l"(gmem), "r"(n), "n"(BYTES) : "memory");
+// Where in a group of sixteen rows of HD bytes (a multiple of 1024 bytes from 0) byte x (a multiple of 4) of row r lies.
+template <int HD> __device__ __forceinline__ int place(int r, int x) {
+  return r * HD + (HD == 128 ? x ^ ((r & 7) << 4) : x ^ (((r >> 1) & 3) << 4));
 }
-template <int WORDS>
-__device__ __forceinline__ void ld_words(uint32_t smem, uint32_t* w) {
-  if constexpr (WORDS == 4) asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(smem));
-  else if constexpr (WORDS == 2) asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(smem));
-  else asm volatile("ld.shared.u32 %0, [%1];" : "=r"(w[0]) : "r"(smem));
+// The key of a group that takes place g (0..7; 8 + g likewise): even places have rows 0, 1, 4, 5, odd ones 3, 2, 7, 6.
+__device__ __forceinline__ int key_at(int g) { return (g & 1) ? ((g & 4) | (3 - ((g >> 1) & 1))) : ((g & 4) | ((g >> 1) & 1)); }
+
+// BYTES (a multiple of 8) from byte x of row r of a group.
+template <int HD, int BYTES>
+__device__ __forceinline__ void read_bytes(const uint8_t* group, int r, int x, uint32_t* w) {
+  if constexpr (BYTES == 8) {
+    const uint2 v = *reinterpret_cast<const uint2*>(group + place<HD>(r, x));
+    w[0] = v.x; w[1] = v.y;
+  } else {
+#pragma unroll
+    for (int i = 0; i < BYTES / 16; ++i) {
+      const uint4 v = *reinterpret_cast<const uint4*>(group + place<HD>(r, x + 16 * i));
+      w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
+    }
+  }
 }
 __device__ __forceinline__ void mma_f16(float* c, const uint32_t* a, uint32_t b0, uint32_t b1) {
   asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -329,11 +343,13 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((((w & 0x7f7
 __device__ __forceinline__ float log2_of(float scale) { return (float)((int)((__float_as_uint(scale) >> 23) & 0xffu) - 127); }
 
 template <int HD, int NB>
-__global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
+__global__ void __launch_bounds__(128, NB == 1 ? Mma<HD>::CTAS : 1)
+kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Attn p) {
   using C = Mma<HD>;
-  constexpr int RT = 8 * NB, NW = C::NW, NG = C::NG, CK = C::CK, KW = C::KB / 4, VW = C::VB / 4;
-  extern __shared__ __align__(16) uint8_t smem[];
-  pdl_trigger();
+  constexpr int RT = 8 * NB, NW = C::NW, NG = C::NG, CK = C::CK, KW = C::KB / 4, VW = C::VB / 4, SLOTS = C::SLOTS;
+  extern __shared__ uint8_t smem_raw[];
+  __shared__ uint64_t full[NW][SLOTS];
+  uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
   const int part = (int)blockIdx.x % p.parts, unit = (int)blockIdx.x / p.parts, kvh = unit % p.kv_heads;
   Tile t;
@@ -343,61 +359,68 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
   if (part >= parts) return;                                   // (a thread that has left counts as arrived at the cluster's barriers)
   const int* bt = p.block_table + (size_t)t.r * p.bt_stride;
   const int stride = parts * NW, first = part * NW + warp;
+  const int mine = first < chunks ? (chunks - 1 - first) / stride + 1 : 0;           // chunks of this warp
+  if (lane == 0) {
+    for (int s = 0; s < SLOTS; ++s) sm100::mbar_init(&full[warp][s], 1);
+    sm100::fence_barrier_init();
+    sm100::tma_prefetch_desc(&map_k);
+    sm100::tma_prefetch_desc(&map_v);
+  }
+  __syncwarp();
 
-  // Lane i looks up the page of group i of a chunk: id, or NONE where nothing of the group is visible.
-  constexpr int NONE = -1, BAD = -2;
-  auto lookup = [&](int c) {
-    const int j = (c_lo + c) * CK + lane * 16;
-    if (lane >= NG || c >= chunks || j >= t.hi || j + 15 < t.lo) return NONE;
+  // The warp's groups are numbered n = 0, 1, ... (chunk n / NG).  Lane i holds what belongs to group 32 b + i: the row of its
+  // first key in the pool (NONE where nothing of it is visible: no page has it, and none of its keys counts), and the page's scales.
+  constexpr int NONE = -1;
+  auto page_of = [&](int n) {
+    const int c = first + (n / NG) * stride, j = (c_lo + c) * CK + (n % NG) * 16;
+    if (c >= chunks || j >= t.hi || j + 15 < t.lo) return NONE;
     const int page = bt[j >> p.page_shift];
-    return page >= 0 && page < p.n_pages ? page : BAD;
-  };
-  const uint32_t ring = sm100::smem_u32(smem) + (uint32_t)(warp * C::STAGES * C::STAGE);
-  const uint8_t* k_lane = p.k_pages + (size_t)g * HD + t4 * C::KB;
-  const uint8_t* v_lane = p.v_pages + (size_t)(2 * t4) * HD + g * C::VB;
-  // Requests chunk c into stage `s`; `page` from lookup(c).  A group without a page is zeros under a scale of 0, which no
-  // page has: none of its keys is visible.
-  auto request = [&](int c, int s, int page) {
-    const uint32_t k_at = ring + (uint32_t)(s * C::STAGE), v_at = k_at + C::K_STAGE, m_at = v_at + C::V_STAGE;
-    long long row = -1;
-    if (lane < NG) {
-      const int j = (c_lo + c) * CK + lane * 16;
-      if (page == BAD) atomicExch(p.status, STATUS_BAD_PAGE_READ);
-      const size_t ph = page >= 0 ? (size_t)page * p.kv_heads + kvh : 0;
-      if (page >= 0) row = (long long)((ph << p.page_shift) + (j & (p.page_size - 1))) * HD;
-      cp_async<4>(m_at + lane * 8, p.k_scales + ph, page >= 0 ? 4 : 0);
-      cp_async<4>(m_at + lane * 8 + 4, p.v_scales + ph, page >= 0 ? 4 : 0);
+    if (page < 0 || page >= p.n_pages) {
+      atomicExch(p.status, STATUS_BAD_PAGE_READ);
+      return NONE;
     }
-#pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      const long long r = __shfl_sync(0xffffffffu, row, i);
-      const bool valid = r >= 0;
-      const uint8_t* kp = k_lane + (valid ? r : 0);            // (zero bytes are read of a group without a page, from page 0)
-      const uint8_t* vp = v_lane + (valid ? r : 0);
-#pragma unroll
-      for (int y = 0; y < 2; ++y)                              // keys g, g + 8
-#pragma unroll
-        for (int x = 0; x < C::KB / C::KP; ++x)
-          cp_async<C::KP>(k_at + (uint32_t)((((2 * i + y) * (C::KB / C::KP) + x) * 32 + lane) * C::KP), kp + y * 8 * HD + x * C::KP,
-                          valid ? C::KP : 0);
-#pragma unroll
-      for (int y = 0; y < 4; ++y)                              // keys 2t, 2t + 1, 2t + 8, 2t + 9
-#pragma unroll
-        for (int x = 0; x < C::VB / C::VP; ++x)
-          cp_async<C::VP>(v_at + (uint32_t)((((4 * i + y) * (C::VB / C::VP) + x) * 32 + lane) * C::VP),
-                          vp + ((y & 1) + 4 * (y & 2)) * HD + x * C::VP, valid ? C::VP : 0);
+    return page;
+  };
+  auto row_of = [&](int n, int page) {
+    const int j = (c_lo + first + (n / NG) * stride) * CK + (n % NG) * 16;
+    return page == NONE ? NONE : (((page * p.kv_heads + kvh) << p.page_shift) | (j & (p.page_size - 1)));
+  };
+  // Requests run SLOTS chunks ahead of the products: `row` is of the 32 groups that are being requested, `ks`, `vs` of the 32 that
+  // are being worked on, `ks_next`, `vs_next` of the former where they differ, `page_ahead` of the 32 behind those.
+  int page = page_of(lane), page_ahead = page_of(32 + lane);
+  int row = row_of(lane, page);
+  float ks_own = 0.f, vs_own = 0.f, ks_next = 0.f, vs_next = 0.f;
+  auto scales_of = [&](int page_, float& ks, float& vs) {      // (0: no page)
+    ks = vs = 0.f;
+    if (page_ != NONE) {
+      ks = p.k_scales[(size_t)page_ * p.kv_heads + kvh];
+      vs = p.v_scales[(size_t)page_ * p.kv_heads + kvh];
     }
   };
-  int pages[C::STAGES];
+  uint8_t* ring = smem + warp * SLOTS * C::SLOT;
+  // Requests the groups of the warp's chunk i.  A group without a page brings row 0 of the pool, which is never looked at.
+  auto request = [&](int i) {
+    const int slot = i % SLOTS;
+    int at[NG];
 #pragma unroll
-  for (int s = 0; s < C::STAGES; ++s) pages[s] = lookup(first + s * stride);
+    for (int y = 0; y < NG; ++y) at[y] = max(0, __shfl_sync(0xffffffffu, row, (i * NG + y) & 31));
+    if (lane == 0) {
+      uint8_t* dst = ring + slot * C::SLOT;
+      sm100::mbar_arrive_expect_tx(&full[warp][slot], C::SLOT);
+#pragma unroll
+      for (int y = 0; y < NG; ++y) {
+        sm100::tma_load_2d(dst + y * C::GROUP, &map_k, 0, at[y], &full[warp][slot]);
+        sm100::tma_load_2d(dst + (NG + y) * C::GROUP, &map_v, 0, at[y], &full[warp][slot]);
+      }
+    }
+  };
+  gb_pin(row);
+  gb_pin(page_ahead);
   pdl_wait();
 #pragma unroll
-  for (int s = 0; s < C::STAGES - 1; ++s) {
-    if (first + s * stride < chunks) request(first + s * stride, s, pages[s]);
-    asm volatile("cp.async.commit_group;" ::: "memory");
-  }
-  int page_next = pages[C::STAGES - 1];
+  for (int i = 0; i < SLOTS; ++i)
+    if (i < mine) request(i);
+  scales_of(page, ks_own, vs_own);
 
   // q: row g of each block, entries t4 * KB ... + KB, under its power of two.  In the lane's columns of S^T and O^T stand rows
   // 2t and 2t + 1 of each block.
@@ -437,15 +460,17 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
 #pragma unroll
     for (int r = 0; r < 2; ++r) {
       factor[b][r] = __shfl_sync(0xffffffffu, back, (2 * t4 + r) * 4);
-      const int mine = 8 * b + 2 * t4 + r;
-      rpos[b][r] = mine < t.rows ? t.pos(mine) : -1;           // (a row that does not exist sees nothing)
+      const int at = 8 * b + 2 * t4 + r;
+      rpos[b][r] = at < t.rows ? t.pos(at) : -1;               // (a row that does not exist sees nothing)
     }
   }
 
-  float m[NB][2], l[NB][2], o[NB][HD / 16][4];
+  // use: what is taken off a row's x: its maximum in use, minus 12 (0 and minus 12 before it has seen anything)
+  float m[NB][2], use[NB][2], l[NB][2], o[NB][HD / 16][4];
 #pragma unroll
   for (int b = 0; b < NB; ++b) {
     m[b][0] = m[b][1] = -INFINITY;
+    use[b][0] = use[b][1] = -12.f;
     l[b][0] = l[b][1] = 0.f;
 #pragma unroll
     for (int n = 0; n < HD / 16; ++n)
@@ -453,122 +478,116 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
       for (int i = 0; i < 4; ++i) o[b][n][i] = 0.f;
   }
   const int pos_first = t.pos(0), pos_last = t.pos(t.rows - 1);
+  const int key_g = key_at(g), key_0 = key_at(2 * t4), key_1 = key_at(2 * t4 + 1);
+  bool alive = true;
 
-  int stage = 0;
-  for (int c = first; c < chunks; c += stride) {
-    asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
-    __syncwarp();                                              // the chunk has landed, and the stage before is free
-    {
-      const int ahead = c + (C::STAGES - 1) * stride;
-      if (ahead < chunks) request(ahead, stage == 0 ? C::STAGES - 1 : stage - 1, page_next);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      page_next = lookup(ahead + stride);
+  for (int i = 0; i < mine; ++i) {
+    const int n0 = i * NG, slot = i % SLOTS;
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(&full[warp][slot], (i / SLOTS) & 1))) {
+      alive = false;
+      break;
     }
-    const uint32_t k_at = ring + (uint32_t)(stage * C::STAGE), v_at = k_at + C::K_STAGE, m_at = v_at + C::V_STAGE;
-    stage = stage == C::STAGES - 1 ? 0 : stage + 1;
-    float s[NB][NG][4], ks[NG], vs[NG];
+    const uint8_t* kt = ring + slot * C::SLOT;
+    const uint8_t* vt = kt + NG * C::GROUP;
+    const int j_chunk = (c_lo + first + i * stride) * CK;
+    float s[NB][NG][4], inv[NG];
     bool careful = false;                                      // some page of the chunk has NaN among its values
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
-      uint32_t sc[2];
-      ld_words<2>(m_at + i * 8, sc);
-      ks[i] = __uint_as_float(sc[0]);
-      vs[i] = __uint_as_float(sc[1]);
-      careful |= vs[i] < 0.f;
+    for (int y = 0; y < NG; ++y) {
+      const float ks = __shfl_sync(0xffffffffu, ks_own, (n0 + y) & 31), vs = __shfl_sync(0xffffffffu, vs_own, (n0 + y) & 31);
+      careful |= vs < 0.f;
+      inv[y] = inverse(vs);
       uint32_t w[2][KW];
 #pragma unroll
-      for (int y = 0; y < 2; ++y)
-#pragma unroll
-        for (int x = 0; x < C::KB / C::KP; ++x)
-          ld_words<C::KP / 4>(k_at + (uint32_t)((((2 * i + y) * (C::KB / C::KP) + x) * 32 + lane) * C::KP), w[y] + x * (C::KP / 4));
+      for (int h = 0; h < 2; ++h) read_bytes<HD, C::KB>(kt + y * C::GROUP, key_g + 8 * h, t4 * C::KB, w[h]);
 #pragma unroll
       for (int b = 0; b < NB; ++b)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[b][i][e] = 0.f;
+        for (int e = 0; e < 4; ++e) s[b][y][e] = 0.f;
 #pragma unroll
       for (int kk = 0; kk < HD / 16; ++kk) {
         uint32_t a[4];
         to_f16(w[0][kk], a[0], a[2]);
         to_f16(w[1][kk], a[1], a[3]);
 #pragma unroll
-        for (int b = 0; b < NB; ++b) mma_f16(s[b][i], a, qb[b][kk][0], qb[b][kk][1]);
+        for (int b = 0; b < NB; ++b) mma_f16(s[b][y], a, qb[b][kk][0], qb[b][kk][1]);
       }
       // x = score + log2(scale of V), -inf where a row does not see the key
-      const int j0 = (c_lo + c) * CK + 16 * i;
-      const bool full = ks[i] != 0.f && j0 + 15 <= pos_first && (p.window <= 0 || j0 + p.window > pos_last);
-      const float lv = log2_of(vs[i]), kf = fabsf(ks[i]);
+      const int j0 = j_chunk + 16 * y;
+      const bool full_ = ks != 0.f && j0 + 15 <= pos_first && (p.window <= 0 || j0 + p.window > pos_last);
+      const float lv = log2_of(vs), kf = fabsf(ks);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const float f0 = factor[b][0] * kf, f1 = factor[b][1] * kf;
-        s[b][i][0] = fmaf(s[b][i][0], f0, lv);
-        s[b][i][1] = fmaf(s[b][i][1], f1, lv);
-        s[b][i][2] = fmaf(s[b][i][2], f0, lv);
-        s[b][i][3] = fmaf(s[b][i][3], f1, lv);
-        if (!full) {
+        s[b][y][0] = fmaf(s[b][y][0], f0, lv);
+        s[b][y][1] = fmaf(s[b][y][1], f1, lv);
+        s[b][y][2] = fmaf(s[b][y][2], f0, lv);
+        s[b][y][3] = fmaf(s[b][y][3], f1, lv);
+        if (!full_) {
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const int j = j0 + g + 8 * (e >> 1), pos = rpos[b][e & 1];
-            const bool seen = ks[i] != 0.f && j <= pos && (p.window <= 0 || j + p.window > pos);
-            s[b][i][e] = seen ? s[b][i][e] : -INFINITY;
+            const int j = j0 + key_g + 8 * (e >> 1), pos = rpos[b][e & 1];
+            const bool seen = ks != 0.f && j <= pos && (p.window <= 0 || j + p.window > pos);
+            s[b][y][e] = seen ? s[b][y][e] : -INFINITY;
           }
         }
       }
     }
     // The maximum in use follows a row's only when it would fall behind by more than 2^3: a weight stays below 2^15.
+    bool grow = false;
+    float top[NB][2];
 #pragma unroll
-    for (int b = 0; b < NB; ++b) {
-      float corr[2];
-      bool grow = false;
+    for (int b = 0; b < NB; ++b)
 #pragma unroll
       for (int r = 0; r < 2; ++r) {
-        float top = fmaxf(s[b][0][r], s[b][0][r + 2]);
+        top[b][r] = fmaxf(s[b][0][r], s[b][0][r + 2]);
 #pragma unroll
-        for (int i = 1; i < NG; ++i) top = fmaxf(top, fmaxf(s[b][i][r], s[b][i][r + 2]));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-        corr[r] = 1.f;
-        if (top > m[b][r] + 3.f || (m[b][r] == -INFINITY && top > -INFINITY)) {
-          corr[r] = ex2(m[b][r] - top);                        // 0 when nothing was seen before
-          m[b][r] = top;
-          l[b][r] *= corr[r];
-          grow = true;
-        }
+        for (int y = 1; y < NG; ++y) top[b][r] = fmaxf(top[b][r], fmaxf(s[b][y][r], s[b][y][r + 2]));
+        grow |= top[b][r] > m[b][r] + 3.f;                     // (m -inf: anything seen)
       }
-      if (grow) {
+    if (__any_sync(0xffffffffu, grow)) {
 #pragma unroll
-        for (int n = 0; n < HD / 16; ++n) {
-          o[b][n][0] *= corr[0]; o[b][n][1] *= corr[1];
-          o[b][n][2] *= corr[0]; o[b][n][3] *= corr[1];
+      for (int b = 0; b < NB; ++b)
+#pragma unroll
+        for (int r = 0; r < 2; ++r) {
+          float top_r = top[b][r];
+#pragma unroll
+          for (int x = 4; x < 32; x *= 2) top_r = fmaxf(top_r, __shfl_xor_sync(0xffffffffu, top_r, x));
+          if (top_r > m[b][r]) {
+            const float corr = ex2(m[b][r] - top_r);           // 0 when nothing was seen before
+            m[b][r] = top_r;
+            use[b][r] = top_r - 12.f;
+            l[b][r] *= corr;
+#pragma unroll
+            for (int n = 0; n < HD / 16; ++n) {
+              o[b][n][r] *= corr;
+              o[b][n][r + 2] *= corr;
+            }
+          }
         }
-      }
     }
 #pragma unroll
-    for (int i = 0; i < NG; ++i) {
+    for (int y = 0; y < NG; ++y) {
       uint32_t pb[NB][2];
-      const float inv = inverse(vs[i]);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
-        const float u0 = (m[b][0] == -INFINITY ? 0.f : m[b][0]) - 12.f, u1 = (m[b][1] == -INFINITY ? 0.f : m[b][1]) - 12.f;
-        const float e0 = ex2(s[b][i][0] - u0), e1 = ex2(s[b][i][1] - u1), e2 = ex2(s[b][i][2] - u0), e3 = ex2(s[b][i][3] - u1);
-        l[b][0] = fmaf(e0 + e2, inv, l[b][0]);
-        l[b][1] = fmaf(e1 + e3, inv, l[b][1]);
-        pb[b][0] = transposed(pack_f16(e0, e1));               // keys 0..7 of the group, then 8..15
+        const float e0 = ex2(s[b][y][0] - use[b][0]), e1 = ex2(s[b][y][1] - use[b][1]);
+        const float e2 = ex2(s[b][y][2] - use[b][0]), e3 = ex2(s[b][y][3] - use[b][1]);
+        l[b][0] = fmaf(e0 + e2, inv[y], l[b][0]);
+        l[b][1] = fmaf(e1 + e3, inv[y], l[b][1]);
+        pb[b][0] = transposed(pack_f16(e0, e1));               // places 0..7 of the group, then 8..15
         pb[b][1] = transposed(pack_f16(e2, e3));
       }
-      uint32_t v[4][VW];
+      uint32_t v[4][VW];                                       // places 2t, 2t + 1, 2t + 8, 2t + 9
 #pragma unroll
-      for (int y = 0; y < 4; ++y)
-#pragma unroll
-        for (int x = 0; x < C::VB / C::VP; ++x)
-          ld_words<C::VP / 4>(v_at + (uint32_t)((((4 * i + y) * (C::VB / C::VP) + x) * 32 + lane) * C::VP), v[y] + x * (C::VP / 4));
-      const int j0 = (c_lo + c) * CK + 16 * i;
+      for (int h = 0; h < 4; ++h) read_bytes<HD, C::VB>(vt + y * C::GROUP, ((h & 1) ? key_1 : key_0) + 4 * (h & 2), g * C::VB, v[h]);
+      const int j0 = j_chunk + 16 * y;
       if (j0 + 16 > t.hi) {                                    // rows behind the context hold anything: 0 * NaN is not 0
 #pragma unroll
-        for (int y = 0; y < 4; ++y)
-          if (j0 + 2 * t4 + (y & 1) + 4 * (y & 2) >= t.hi) {
+        for (int h = 0; h < 4; ++h)
+          if (j0 + ((h & 1) ? key_1 : key_0) + 4 * (h & 2) >= t.hi) {
 #pragma unroll
-            for (int w = 0; w < VW; ++w) v[y][w] = 0u;
+            for (int w = 0; w < VW; ++w) v[h][w] = 0u;
           }
       }
       if (careful) {
@@ -578,15 +597,15 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
 #pragma unroll
         for (int b = 0; b < NB; ++b)
 #pragma unroll
-          for (int y = 0; y < 2; ++y)
-            see[b][y] = transposed(pack_f16(s[b][i][2 * y] == -INFINITY ? 0.f : 1.f, s[b][i][2 * y + 1] == -INFINITY ? 0.f : 1.f));
+          for (int h = 0; h < 2; ++h)
+            see[b][h] = transposed(pack_f16(s[b][y][2 * h] == -INFINITY ? 0.f : 1.f, s[b][y][2 * h + 1] == -INFINITY ? 0.f : 1.f));
 #pragma unroll
         for (int w = 0; w < VW; ++w) {
           uint32_t bad[4];
 #pragma unroll
-          for (int y = 0; y < 4; ++y) {
-            bad[y] = nan_bytes(v[y][w]);
-            v[y][w] &= ~bad[y];
+          for (int h = 0; h < 4; ++h) {
+            bad[h] = nan_bytes(v[h][w]);
+            v[h][w] &= ~bad[h];
           }
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
@@ -618,8 +637,26 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
           for (int b = 0; b < NB; ++b) mma_f16(o[b][2 * w + h], a, pb[b][0], pb[b][1]);
         }
     }
+    __syncwarp();                                              // every lane has read the slot
+    const int ahead = i + SLOTS;
+    if (ahead < mine) {
+      if (((ahead * NG) & 31) == 0) {
+        row = row_of(ahead * NG + lane, page_ahead);
+        scales_of(page_ahead, ks_next, vs_next);
+        page_ahead = page_of(ahead * NG + 32 + lane);
+      }
+      request(ahead);
+    }
+    if (((n0 + NG) & 31) == 0) {
+      ks_own = ks_next;
+      vs_own = vs_next;
+    }
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  pdl_trigger();       // (not earlier: CTAs of the next kernel beside these would leave its others unevenly spread over the SMs)
+  if (!alive) {
+    if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT);
+    for (int i = 0; i < 1000; ++i) __nanosleep(1000);          // copies still in flight land before the memory is used again
+  }
   __syncthreads();                                             // the rings are no longer read
   float* m_s = reinterpret_cast<float*>(smem);                 // [NW + 1][RT], [RT] sums of the CTA
   float* l_s = m_s + (NW + 2) * RT;                            // [NW][RT]
@@ -647,8 +684,8 @@ __global__ void __launch_bounds__(128) kv8_attention_mma_kernel(const Attn p) {
 // ---------------------------------------------------------------- launches
 // Launches `kernel` over the tiles, their kv heads and parts (x in this order, parts fastest: the tiles with the most keys of
 // every head start first), a tile's parts as a cluster.
-template <typename K>
-int launch_parts(K kernel, Attn p, int parts, long long tiles, int threads, size_t smem, cudaStream_t stream) {
+template <typename K, typename... Maps>
+int launch_parts(K kernel, Attn p, int parts, long long tiles, int threads, size_t smem, cudaStream_t stream, const Maps&... maps) {
   p.parts = parts;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(tiles * p.kv_heads * parts));
@@ -669,7 +706,7 @@ int launch_parts(K kernel, Attn p, int parts, long long tiles, int threads, size
   }
   cfg.attrs = attr;
   cfg.numAttrs = n;
-  GB_CUDA(cudaLaunchKernelEx(&cfg, kernel, p));
+  GB_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps..., p));
   return GB_OK;
 }
 
@@ -702,27 +739,34 @@ int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t st
   }
 }
 
+// The pool of pages [rows, HD] as a tensor map whose copies are groups of sixteen rows.
+template <int HD>
+bool group_map(CUtensorMap* map, const void* pages, long long rows) {
+  const TensorMapFn fn = tensor_map_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)HD};
+  const cuuint32_t box[2] = {(cuuint32_t)HD, 16}, step[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pages), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <int HD, int NB>
 int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
   using C = Mma<HD>;
-  constexpr int SMEM = C::smem(8 * NB), SLOTS = 227 * 1024 / (SMEM + 1024) < 4 ? 227 * 1024 / (SMEM + 1024) : 4;
+  constexpr int SMEM = C::smem(8 * NB);
   static bool attr_set = false;
   if (!attr_set) {
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set = true;
   }
-  return launch_parts(kv8_attention_mma_kernel<HD, NB>, p, key_parts(tiles * p.kv_heads, 148 * SLOTS, (keys + C::CK - 1) / C::CK, C::NW),
-                      tiles, 32 * C::NW, SMEM, stream);
-}
-template <int NB>
-int dispatch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
-  switch (p.hd) {
-    case 32: return launch_mma<32, NB>(p, tiles, keys, stream);
-    case 64: return launch_mma<64, NB>(p, tiles, keys, stream);
-    case 96: return launch_mma<96, NB>(p, tiles, keys, stream);
-    default: return launch_mma<128, NB>(p, tiles, keys, stream);
-  }
+  CUtensorMap mk, mv;
+  const long long rows = (long long)p.n_pages * p.kv_heads * p.page_size;
+  if (!group_map<HD>(&mk, p.k_pages, rows) || !group_map<HD>(&mv, p.v_pages, rows))
+    GB_FAIL(GB_ERR_CUDA, "kv8_attention: cuTensorMapEncodeTiled failed (%lld rows of %d)", rows, HD);
+  const int parts = key_parts(tiles * p.kv_heads, 148 * C::CTAS, (keys + C::CK - 1) / C::CK, C::NW);
+  return launch_parts(kv8_attention_mma_kernel<HD, NB>, p, parts, tiles, 32 * C::NW, SMEM, stream, mk, mv);
 }
 
 }  // namespace
@@ -758,8 +802,8 @@ GB_OP(gb_op_kv8_attention) {
   const int group = p.heads / p.kv_heads;
   p.page_shift = 0;
   while ((1 << p.page_shift) < p.page_size) ++p.page_shift;
-  const bool mma = dtype == GB_BF16 && (p.hd == 32 || p.hd == 64 || p.hd == 96 || p.hd == 128) && p.page_size >= 16 &&
-                   (1 << p.page_shift) == p.page_size && p.ldq % 8 == 0 && ((uintptr_t)p.q & 15) == 0;
+  const bool mma = dtype == GB_BF16 && (p.hd == 64 || p.hd == 128) && p.page_size >= 16 &&
+                   (1 << p.page_shift) == p.page_size && (long long)p.n_pages * p.kv_heads * p.page_size < 0x7fffffff && p.ldq % 8 == 0 && ((uintptr_t)p.q & 15) == 0;
   // rows of a tile: with 8, a step of single tokens in groups of eight heads or fewer; with 16, half as many passes over the keys
   const bool small = (long long)p.step.max_q * group <= 8;
   // upper bound of the tiles: sum_r ceil(q_len_r * group / rt)
@@ -770,7 +814,8 @@ GB_OP(gb_op_kv8_attention) {
   const long long keys = p.window > 0 && p.window + rt < p.step.max_ctx ? p.window + rt : p.step.max_ctx;
   int rc;
   if (mma)
-    rc = small ? dispatch_mma<1>(p, tiles, keys, ctx->stream) : dispatch_mma<2>(p, tiles, keys, ctx->stream);
+    rc = p.hd == 64 ? (small ? launch_mma<64, 1>(p, tiles, keys, ctx->stream) : launch_mma<64, 2>(p, tiles, keys, ctx->stream))
+                    : (small ? launch_mma<128, 1>(p, tiles, keys, ctx->stream) : launch_mma<128, 2>(p, tiles, keys, ctx->stream));
   else
     rc = dtype == GB_F32 ? dispatch_any<float>(p, tiles, keys, ctx->stream) : dispatch_any<bf16>(p, tiles, keys, ctx->stream);
   if (rc != GB_OK) return rc;
