@@ -36,7 +36,7 @@ LIBRARIES = {
                "sigmoid_attention_tc.cu", "ssm.cu", "selective_scan.cu", "delta_rule.cu", "delta_chunks.cu", "linear_scan.cu", "streams.cu", "moe.cu",
                "moe_tc.cu"],
     # the 8-bit paged cache: storing, attention, and copies of rows of any cache (forked requests)
-    "kv8": ["errors.cu", "kv8_store.cu", "kv8_attention.cu", "row_copies.cu"],
+    "kv8": ["errors.cu", "kv8_store.cu", "kv8_attention.cu", "kv8_attention_tcgen05.cu", "kv8_call.cu", "row_copies.cu"],
 }
 
 NVCC_FLAGS = [

@@ -10,27 +10,13 @@
 // a0 q rows, a1 their stride, a2 dtype (of q and out), a3 out, a4 its stride, a5 k pages, a6 v pages, a7 k scales, a8 v
 // scales, a9 pages, a10 page size, a11 heads, a12 kv heads, a13 hd, a14 block table, a15 its stride, a16 window (0: none);
 // f0 scale.  The step's requests come from its symbols.
-#include "kv8.cuh"
-#include "sm100.cuh"
+#include "kv8_attention.cuh"
 
 namespace {
 
 using namespace kv8;
 
-struct Attn {
-  const void* q; long long ldq;
-  void* out; long long ldo;
-  const uint8_t* k_pages; const uint8_t* v_pages; const float* k_scales; const float* v_scales;
-  int n_pages, page_size, heads, kv_heads, hd, window;
-  const int* block_table; int bt_stride;
-  Step step;
-  int parts;                         // CTAs of a cluster
-  int page_shift;                    // log2 of the page size, where that is a power of two
-  float scale_log2;                  // scale * log2(e)
-  int* status;
-};
-
-constexpr int STATUS_TIMEOUT = 40;   // a bounded wait ran out
+constexpr int FEW = 32;              // rows of a request up to which it is not worth 256-row tiles
 constexpr int MAX_PARTS = 16;        // CTAs of a cluster that share a tile's keys, at most (8 is the portable limit)
 
 // A tile's request, rows and keys.
@@ -46,7 +32,10 @@ __device__ __forceinline__ bool find_tile(const Attn& p, int index, Tile& t) {
   t.group = p.heads / p.kv_heads;
   int tile = 0;
   t.r = find_piece(index, p.step.n_requests, true,
-                   [&](int i) { return (p.step.q_len[i] * t.group + RT - 1) / RT; }, tile);
+                   [&](int i) {
+                     const int rows = p.step.q_len[i] * t.group;
+                     return rows > p.few ? 0 : (rows + RT - 1) / RT;
+                   }, tile);
   if (t.r < 0) return false;
   const int qlen = p.step.q_len[t.r];
   const int tiles = (qlen * t.group + RT - 1) / RT;
@@ -60,11 +49,6 @@ __device__ __forceinline__ bool find_tile(const Attn& p, int index, Tile& t) {
   return true;
 }
 
-__device__ __forceinline__ uint32_t cluster_addr(const void* p, int rank) {
-  uint32_t a;
-  asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(sm100::smem_u32(p)), "r"(rank));
-  return a;
-}
 __device__ __forceinline__ float ld_cluster(const float* p, int rank) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(cluster_addr(p, rank)) : "memory");
@@ -100,7 +84,7 @@ __device__ __forceinline__ void join(const Attn& p, const Tile& t, int kvh, int 
     if (parts == 1) {
       const int tok = (t.row0 + r) / t.group, g = (t.row0 + r) - tok * t.group;
       reinterpret_cast<T*>(p.out)[(size_t)(t.qstart + tok) * p.ldo + (size_t)(kvh * t.group + g) * hd + d] =
-          from_f32<T>(acc / cl[r]);
+          from_f32<T>(cl[r] != 0.f ? acc / cl[r] : 0.f);
     } else {
       o[(size_t)r * hd + d] = acc;                             // (warp 0's place, read by this thread only)
     }
@@ -124,7 +108,7 @@ __device__ __forceinline__ void join(const Attn& p, const Tile& t, int kvh, int 
       acc = fmaf(f, ld_cluster(o + (size_t)r * hd + d, z), acc);
     }
     const int tok = (t.row0 + r) / t.group, g = (t.row0 + r) - tok * t.group;
-    reinterpret_cast<T*>(p.out)[(size_t)(t.qstart + tok) * p.ldo + (size_t)(kvh * t.group + g) * hd + d] = from_f32<T>(acc / sum);
+    reinterpret_cast<T*>(p.out)[(size_t)(t.qstart + tok) * p.ldo + (size_t)(kvh * t.group + g) * hd + d] = from_f32<T>(sum != 0.f ? acc / sum : 0.f);
   }
   sm100::cluster_sync_all();                                   // nobody leaves while another CTA reads its share
 }
@@ -323,25 +307,6 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8 x 8 matri
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-__device__ __forceinline__ float ex2(float x) {                // relative error 2^-22; -inf gives 0
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  uint32_t r;
-  asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-  return r;
-}
-// Bytes 0, 1 (2, 3) of a word as two f16.
-__device__ __forceinline__ void to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
-  asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}" : "=r"(lo), "=r"(hi) : "r"(w));
-}
-// 0xff in the bytes that are NaN.
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u) >> 7) * 255u; }
-// log2 and inverse of a power of two (the sign does not matter)
-__device__ __forceinline__ float log2_of(float scale) { return (float)((int)((__float_as_uint(scale) >> 23) & 0xffu) - 127); }
-
 template <int HD, int NB>
 __global__ void __launch_bounds__(128, NB == 1 ? Mma<HD>::CTAS : 1)
 kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Attn p) {
@@ -682,34 +647,6 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
 }
 
 // ---------------------------------------------------------------- launches
-// Launches `kernel` over the tiles, their kv heads and parts (x in this order, parts fastest: the tiles with the most keys of
-// every head start first), a tile's parts as a cluster.
-template <typename K, typename... Maps>
-int launch_parts(K kernel, Attn p, int parts, long long tiles, int threads, size_t smem, cudaStream_t stream, const Maps&... maps) {
-  p.parts = parts;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(tiles * p.kv_heads * parts));
-  cfg.blockDim = dim3((unsigned)threads);
-  cfg.dynamicSmemBytes = smem;
-  cfg.stream = stream;
-  cudaLaunchAttribute attr[2];
-  int n = 0;
-  if (gb_pdl_enabled()) {
-    attr[n].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[n++].val.programmaticStreamSerializationAllowed = 1;
-  }
-  if (parts > 1) {
-    attr[n].id = cudaLaunchAttributeClusterDimension;
-    attr[n].val.clusterDim.x = (unsigned)parts;
-    attr[n].val.clusterDim.y = 1;
-    attr[n++].val.clusterDim.z = 1;
-  }
-  cfg.attrs = attr;
-  cfg.numAttrs = n;
-  GB_CUDA(cudaLaunchKernelEx(&cfg, kernel, maps..., p));
-  return GB_OK;
-}
-
 // How many CTAs share a tile's keys: as many as fill `slots` places on the GPU, each with a chunk for every warp.
 int key_parts(long long ctas, long long slots, long long chunks, int warps) {
   int parts = 1;
@@ -771,6 +708,8 @@ int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stre
 
 }  // namespace
 
+int kv8_attention_tcgen05(const kv8::Attn& p, cudaStream_t stream);      // kv8_attention_tcgen05.cu
+
 GB_OP(gb_op_kv8_attention) {
   (void)flags;
   Attn p;
@@ -804,12 +743,28 @@ GB_OP(gb_op_kv8_attention) {
   while ((1 << p.page_shift) < p.page_size) ++p.page_shift;
   const bool mma = dtype == GB_BF16 && (p.hd == 64 || p.hd == 128) && p.page_size >= 16 &&
                    (1 << p.page_shift) == p.page_size && (long long)p.n_pages * p.kv_heads * p.page_size < 0x7fffffff && p.ldq % 8 == 0 && ((uintptr_t)p.q & 15) == 0;
-  // rows of a tile: with 8, a step of single tokens in groups of eight heads or fewer; with 16, half as many passes over the keys
-  const bool small = (long long)p.step.max_q * group <= 8;
+  // Requests of more than FEW rows go to tcgen05, which takes 256 rows at a time; they have to lie on 16-byte boundaries.
+  const bool wide = mma && (long long)p.step.max_q * group > FEW && group <= 64 && p.ldo % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
+  p.few = 0x7fffffff;
+  int launched = 0;
+  if (wide) {
+    p.few = p.step.n_requests == 1 ? 0 : FEW;                  // (one request: all of it, whatever it brings)
+    const int rc = kv8_attention_tcgen05(p, ctx->stream);
+    if (rc != GB_OK) return rc;
+    if (p.step.n_requests == 1) return 1;
+    launched = 1;
+  }
+  // rows of a tile: with 8, a step of single tokens in groups of eight heads or fewer, and what stands beside wide portions (single
+  // tokens as a rule); with 16, half as many passes over the keys
+  const bool small = wide || (long long)p.step.max_q * group <= 8;
   // upper bound of the tiles: sum_r ceil(q_len_r * group / rt)
   const int rt = !mma ? 4 : small ? 8 : 16;
-  const long long tiles = p.step.one_each ? (long long)p.step.n_requests * ((group + rt - 1) / rt)
-                                          : (long long)p.step.n_tokens * group / rt + p.step.n_requests;
+  long long tiles = p.step.one_each ? (long long)p.step.n_requests * ((group + rt - 1) / rt)
+                                    : (long long)p.step.n_tokens * group / rt + p.step.n_requests;
+  if (wide) {                                                  // (the requests that are left have FEW rows at most)
+    const long long most = (long long)p.step.n_requests * ((FEW + rt - 1) / rt);
+    tiles = tiles < most ? tiles : most;
+  }
   if (tiles * p.kv_heads > 0x7fffffff / MAX_PARTS) GB_FAIL(GB_ERR_ARG, "kv8_attention: %lld tiles in one launch", tiles);
   const long long keys = p.window > 0 && p.window + rt < p.step.max_ctx ? p.window + rt : p.step.max_ctx;
   int rc;
@@ -820,5 +775,5 @@ GB_OP(gb_op_kv8_attention) {
     rc = dtype == GB_F32 ? dispatch_any<float>(p, tiles, keys, ctx->stream) : dispatch_any<bf16>(p, tiles, keys, ctx->stream);
   if (rc != GB_OK) return rc;
   GB_CHECK_LAUNCH("kv8_attention");
-  return 1;
+  return launched + 1;
 }

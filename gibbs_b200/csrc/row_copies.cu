@@ -84,15 +84,23 @@ int check_pairs(int g, const int* pairs, int n, int rows) {
 
 GB_API int gb_row_copies_piece_bytes() { return 4096; }
 
-// pieces: device memory, one record of three 64-bit words (address in row 0, bytes between rows, bytes) each, group after
-// group; n_pieces, n_rows [n_groups]; pairs [sum of n_pairs] (src, dst) in host memory, group after group; n_pairs [n_groups].
+// What a call needs in one array of 64-bit words: w0 the pieces (device memory, one record of three words each: address in row
+// 0, bytes between rows, bytes; group after group), w1 stream, w2 groups, then for each group its pairs (host memory, (src, dst)
+// as 32-bit integers) and their number, then for each group its pieces and rows.
 // Every source is read as it was before the call: a row that is a destination twice, or a destination and a source, is
 // refused, as is a row outside the group.  Returns the number of kernels launched, or a negative error code.
-GB_API int gb_row_copies(const void* pieces, int n_groups, const int* n_pieces, const int* n_rows, const int* const* pairs,
-                         const int* n_pairs, cudaStream_t stream) {
+GB_API int gb_row_copies(const long long* w) {
+  const void* pieces = reinterpret_cast<const void*>(w[0]);
+  cudaStream_t stream = reinterpret_cast<cudaStream_t>(w[1]);
+  const int n_groups = (int)w[2];
   if (n_groups < 0 || n_groups > MAX_GROUPS) GB_FAIL(GB_ERR_ARG, "row copies: %d groups, %d at most", n_groups, MAX_GROUPS);
+  const int* pairs[MAX_GROUPS];
+  int n_pairs[MAX_GROUPS], n_pieces[MAX_GROUPS];
   for (int g = 0; g < n_groups; ++g) {
-    int rc = check_pairs(g, pairs[g], n_pairs[g], n_rows[g]);
+    pairs[g] = reinterpret_cast<const int*>(w[3 + 2 * g]);
+    n_pairs[g] = (int)w[4 + 2 * g];
+    n_pieces[g] = (int)w[3 + 2 * n_groups + 2 * g];
+    const int rc = check_pairs(g, pairs[g], n_pairs[g], (int)w[4 + 2 * n_groups + 2 * g]);
     if (rc != GB_OK) return rc;
   }
   int launched = 0;

@@ -61,6 +61,17 @@ def _stream():
     return _c_void(torch.cuda.current_stream().cuda_stream)
 
 
+def raw_stream(device: torch.device) -> int:
+    """The handle of the current stream of ``device``, which has to be the current device (or of the stream a
+    ``launching_on`` block is active for)."""
+    if _STREAM is not None:
+        return _STREAM.value or 0
+    index = torch.cuda.current_device()
+    if device.index != index:
+        raise KernelError(f"the tensors lie on {device}, the current device is cuda:{index}")
+    return torch._C._cuda_getCurrentRawStream(index)
+
+
 class launching_on:
     """Within the block every kernel of this module launches on ``stream`` (default: the
     current CUDA stream at entry) without asking torch for the current stream at every

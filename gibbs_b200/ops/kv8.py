@@ -15,11 +15,12 @@ before the kernel in front of the call begins: kernels read it ahead of what tha
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Optional
 
 import torch
 
-from . import _f32vec, _i32, _launched, _need_cuda, _rotary_table, _rows, _stream, device_status, dtype_code
+from . import _f32vec, _launched, _need_cuda, _rotary_table, _rows, device_status, dtype_code, raw_stream
 from .library import KernelError, check, library
 
 LIBRARY = "kv8"
@@ -28,15 +29,9 @@ DTYPE = torch.float8_e4m3fn
 TAKES_PARTIALS = 1 << 29         # a record's flag: the operation adds the partial tiles of the product in front
 MAX_HEAD_DIM = 256
 
-_A, _F, _SYM = ctypes.c_longlong * 24, ctypes.c_double * 3, ctypes.c_longlong * 32
-
-
-class _Ctx(ctypes.Structure):
-    _fields_ = [("stream", ctypes.c_void_p), ("status", ctypes.c_void_p), ("sym", ctypes.c_void_p),
-                ("n_sym", ctypes.c_int), ("residual", ctypes.c_void_p), ("residual_ld", ctypes.c_longlong),
-                ("pend", ctypes.c_void_p), ("pend_splits", ctypes.c_int), ("pend_bias", ctypes.c_void_p),
-                ("part", ctypes.c_void_p), ("part_splits", ctypes.c_int), ("part_bias", ctypes.c_void_p)]
-
+# what csrc/kv8_call.cu reads: operation, stream, status word, twelve symbols, partial tiles, their number and bias; the
+# floating operand; twenty operands
+_WORDS = struct.Struct("=18qd20q")
 
 _FN: dict = {}
 _IDS: dict = {}
@@ -94,34 +89,34 @@ def check_head_dim(head_dim: int) -> None:
         raise KernelError(f"an 8-bit cache holds heads of a multiple of 8 entries up to {MAX_HEAD_DIM}, not {head_dim}")
 
 
-def _call(name: str, device: torch.device, a, f0: float, step, part=None) -> None:
-    if device.index != torch.cuda.current_device():
-        raise KernelError(f"{name}: the tensors lie on {device}, the current device is cuda:{torch.cuda.current_device()}")
+def _call(operation: int, device: torch.device, a, f0: float, step, part=None) -> None:
+    run = _FN.get("run")
+    if run is None:
+        run = _FN["run"] = library(LIBRARY).gb_kv8_run
+        run.argtypes, run.restype = [ctypes.c_char_p], ctypes.c_int
     n, r, longest = step.n_tokens, step.n_requests, step.max_q_len
-    sym = _SYM(n, r, 0, longest, step.max_ctx_len, 1 if longest == 1 and n == r else 0, 0, 0, 0, step.q_start.data_ptr(),
-               step.q_len.data_ptr(), step.start_pos.data_ptr())
-    stream = _stream()
-    ctx = _Ctx(stream.value if isinstance(stream, ctypes.c_void_p) else stream, device_status(device).data_ptr(),
-               ctypes.addressof(sym), 32)
-    flags = 0
+    ws, splits, bias = 0, 0, 0
     if part is not None:
-        flags = TAKES_PARTIALS
-        ctx.part, ctx.part_splits = part.ws.data_ptr(), part.ws.shape[0]
-        ctx.part_bias = None if part.bias is None else part.bias.data_ptr()
-    rc = (_FN.get(name) or _function(name))(ctypes.byref(ctx), _A(*a), _F(f0), flags)
+        ws, splits, bias = part.ws.data_ptr(), part.ws.shape[0], 0 if part.bias is None else part.bias.data_ptr()
+    rc = run(_WORDS.pack(operation, raw_stream(device), device_status(device).data_ptr(), n, r, 0, longest, step.max_ctx_len,
+                         1 if longest == 1 and n == r else 0, 0, 0, 0, step.q_start.data_ptr(), step.q_len.data_ptr(),
+                         step.start_pos.data_ptr(), ws, splits, bias, f0, *a))
     if rc < 0:
         check(library(LIBRARY), rc)
     _launched(rc)
 
 
-def _check_step(step, block_table: torch.Tensor, rows: int, what: str) -> None:
-    _need_cuda(block_table, step.q_start, step.q_len, step.start_pos)
-    for t, name in ((step.q_start, "q_start"), (step.q_len, "q_len"), (step.start_pos, "start_pos")):
-        if t.dtype != torch.int32 or not t.is_contiguous() or t.numel() < step.n_requests:
-            raise KernelError(f"{what} {name}: {step.n_requests} contiguous int32 values expected")
-    if block_table.dtype != torch.int32 or block_table.dim() != 2 or not block_table.is_contiguous() \
-            or block_table.shape[0] < step.n_requests:
-        raise KernelError(f"{what}: the block table is contiguous int32 [{step.n_requests} requests, entries]")
+_I32 = torch.int32
+
+
+def _check_step(step, block_table: torch.Tensor, rows: int, device: torch.device, what: str) -> None:
+    n = step.n_requests
+    for t in (step.q_start, step.q_len, step.start_pos):
+        if t.dtype is not _I32 or t.device != device or not t.is_contiguous() or t.numel() < n:
+            raise KernelError(f"{what}: q_start, q_len and start_pos are {n} contiguous int32 values on {device}")
+    if block_table.dtype is not _I32 or block_table.device != device or block_table.dim() != 2 \
+            or not block_table.is_contiguous() or block_table.shape[0] < n:
+        raise KernelError(f"{what}: the block table is contiguous int32 [{n} requests, entries] on {device}")
     if rows < step.n_tokens:
         raise KernelError(f"{what}: {rows} rows, the step has {step.n_tokens} tokens")
 
@@ -158,7 +153,7 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
     if inv_freq is not None and (rotary_dim % 2 or not 0 <= rotary_dim <= head_dim):
         raise KernelError(f"kv8 store: a rotation over {rotary_dim} of {head_dim} entries")
     table = _rotary_table(inv_freq, rotary_dim)
-    _check_step(step, block_table, rows, "kv8 store")
+    _check_step(step, block_table, rows, x.device, "kv8 store")
     if pages is not None:
         if (pages.kv_heads, pages.head_dim) != (kv_heads, head_dim) or pages.device != x.device:
             raise KernelError(f"kv8 store: the pages hold {pages.kv_heads} kv heads of {pages.head_dim} on {pages.device}")
@@ -167,11 +162,11 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
     else:
         k = v = ks = vs = n_pages = 0
         page_size = 16
-    a = (0 if part is not None else x.data_ptr(), ld, code, q_out.data_ptr(), 0 if q_gain is None else q_gain.data_ptr(),
+    a = (x.data_ptr() if part is None else 0, ld, code, q_out.data_ptr(), 0 if q_gain is None else q_gain.data_ptr(),
          0 if k_gain is None else k_gain.data_ptr(), 0 if table is None else table.data_ptr(), rotary_dim if table is not None else 0,
          1 if adjacent_pairs else 0, k, v, ks, vs, n_pages, page_size, heads, kv_heads, head_dim, block_table.data_ptr(),
          block_table.shape[1])
-    _call("kv8_store", x.device, a, eps, step, part)
+    _call(0, x.device, a, eps, step, part)
     return q_out
 
 
@@ -182,16 +177,17 @@ def paged_attention(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, p
     _need_cuda(q, out)
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
         raise KernelError(f"kv8 attention: {heads} heads are not a multiple of {kv_heads} kv heads")
-    cols = heads * head_dim
+    cols, device = heads * head_dim, q.device
     if q.dim() != 2 or out.dim() != 2 or q.shape[1] != cols or out.shape[1] != cols or q.dtype != out.dtype \
             or out.shape[0] < step.n_tokens:
         raise KernelError(f"kv8 attention: q and out are [tokens, {cols}] of one dtype")
-    if (pages.kv_heads, pages.head_dim) != (kv_heads, head_dim) or pages.device != q.device or out.device != q.device:
+    if pages.kv_heads != kv_heads or pages.head_dim != head_dim or pages.device != device or out.device != device:
         raise KernelError(f"kv8 attention: the pages hold {pages.kv_heads} kv heads of {pages.head_dim} on {pages.device}")
     if window is None or window < 0:
         raise KernelError(f"kv8 attention: a window of {window} keys (0: none)")
-    _check_step(step, block_table, q.shape[0], "kv8 attention")
-    a = (q.data_ptr(), _rows(q, "q"), dtype_code(q.dtype), out.data_ptr(), _rows(out, "out"), *pages.addresses, pages.n_pages,
-         pages.page_size, heads, kv_heads, head_dim, block_table.data_ptr(), block_table.shape[1], window)
-    _call("kv8_attention", q.device, a, scale, step)
+    _check_step(step, block_table, q.shape[0], device, "kv8 attention")
+    k, v, ks, vs = pages.addresses
+    _call(1, device, (q.data_ptr(), _rows(q, "q"), dtype_code(q.dtype), out.data_ptr(), _rows(out, "out"), k, v, ks, vs,
+                      pages.n_pages, pages.page_size, heads, kv_heads, head_dim, block_table.data_ptr(), block_table.shape[1],
+                      window, 0, 0, 0), scale, step)
     return out

@@ -2,11 +2,12 @@
 from __future__ import annotations
 
 import ctypes
+import struct
 from typing import Sequence
 
 import torch
 
-from . import _launched, _stream
+from . import _launched, raw_stream
 from .library import KernelError, check, library
 
 LIBRARY = "kv8"
@@ -45,8 +46,10 @@ class RowCopies:
             n_pieces.append(len(records) - before)
         self._pieces = torch.tensor(records or [(0, 0, 0)], dtype=torch.int64).to(self.device)
         n = len(self.groups)
-        self._n_pieces = (ctypes.c_int * n)(*n_pieces)
-        self._n_rows = (ctypes.c_int * n)(*[g[0].shape[0] for g in self.groups])
+        self._table, self._sizes = self._pieces.data_ptr(), [v for i, g in enumerate(self.groups) for v in (n_pieces[i], g[0].shape[0])]
+        self._format = f"={3 + 4 * n}q"
+        self._run = lib.gb_row_copies
+        self._run.argtypes, self._run.restype = [ctypes.c_char_p], ctypes.c_int
         torch.cuda.current_stream(self.device).synchronize()       # the records lie in place whatever stream copies use
 
     def copy(self, pairs: Sequence) -> int:
@@ -55,28 +58,25 @@ class RowCopies:
         refused, and then nothing is copied.  Launches on the current stream; returns the number of kernels."""
         if len(pairs) != len(self.groups):
             raise KernelError(f"row copies: pairs for {len(pairs)} groups, {len(self.groups)} expected")
-        if self.device.index != torch.cuda.current_device():
-            raise KernelError(f"row copies: the tensors lie on {self.device}, the current device is cuda:{torch.cuda.current_device()}")
-        keep, at, counts = [], [], []
+        keep, words = [], []
         for i, p in enumerate(pairs):
             if isinstance(p, torch.Tensor):
                 if p.is_cuda or p.dtype != torch.int32 or p.dim() != 2 or p.shape[1] != 2 or not p.is_contiguous():
                     raise KernelError(f"row copies: pairs of group {i} are contiguous int32 [n, 2] on the host")
                 keep.append(p)
-                at.append(p.data_ptr())
+                words += (p.data_ptr(), len(p))
             else:
-                flat = []
-                for src, dst in p:
-                    flat += (src, dst)
-                if any(not -(1 << 31) <= v < 1 << 31 for v in flat):
-                    raise KernelError(f"row copies: a row of group {i} outside 32 bits")
-                keep.append((ctypes.c_int * max(1, len(flat)))(*flat))
-                at.append(ctypes.addressof(keep[-1]))
-            counts.append(len(p))
-        lib, n = library(LIBRARY), len(at)
-        rc = lib.gb_row_copies(ctypes.c_void_p(self._pieces.data_ptr()), n, self._n_pieces, self._n_rows,
-                               (ctypes.c_void_p * n)(*at), (ctypes.c_int * n)(*counts), _stream())
+                flat = [v for pair in p for v in pair]
+                try:
+                    a = (ctypes.c_int * len(flat)).from_buffer_copy(struct.pack(f"={len(flat)}i", *flat)) if flat else None
+                except struct.error as e:
+                    raise KernelError(f"row copies: pairs of group {i} are 32-bit integers ({e})") from None
+                if len(flat) != 2 * len(p):
+                    raise KernelError(f"row copies: pairs of group {i} are (src, dst)")
+                keep.append(a)
+                words += (0 if a is None else ctypes.addressof(a), len(p))
+        rc = self._run(struct.pack(self._format, self._table, raw_stream(self.device), len(self.groups), *words, *self._sizes))
         if rc < 0:
-            check(lib, rc)
+            check(library(LIBRARY), rc)
         _launched(rc)
         return rc

@@ -1,6 +1,7 @@
 """What the 8-bit cache and the row copies refuse, as far as it needs no GPU."""
 import ctypes
 import math
+import struct
 
 import pytest
 import torch
@@ -46,9 +47,8 @@ def test_pairs_are_checked_before_anything_is_launched(pairs):
     lib = library("kv8")
     n, flat = len(pairs), [v for p in pairs for v in p]
     arr = (ctypes.c_int * len(flat))(*flat)
-    one = lambda v: (ctypes.c_int * 1)(v)                                                              # noqa: E731
-    rc = lib.gb_row_copies(ctypes.c_void_p(0), 1, one(1), one(10), (ctypes.c_void_p * 1)(ctypes.addressof(arr)), one(n), ctypes.c_void_p(0))
-    assert rc < 0
+    lib.gb_row_copies.argtypes, lib.gb_row_copies.restype = [ctypes.c_char_p], ctypes.c_int
+    assert lib.gb_row_copies(struct.pack("=7q", 0, 0, 1, ctypes.addressof(arr), n, 1, 10)) < 0
     lib.gb_last_error.restype = ctypes.c_char_p
     assert b"row copies" in lib.gb_last_error()
 
