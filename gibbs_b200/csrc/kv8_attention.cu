@@ -676,18 +676,6 @@ int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t st
   }
 }
 
-// The pool of pages [rows, HD] as a tensor map whose copies are groups of sixteen rows.
-template <int HD>
-bool group_map(CUtensorMap* map, const void* pages, long long rows) {
-  const TensorMapFn fn = tensor_map_fn();
-  if (!fn) return false;
-  const cuuint64_t dims[2] = {(cuuint64_t)HD, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)HD};
-  const cuuint32_t box[2] = {(cuuint32_t)HD, 16}, step[2] = {1, 1};
-  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pages), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-            HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B, CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
-            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
-}
-
 template <int HD, int NB>
 int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
   using C = Mma<HD>;
@@ -700,7 +688,8 @@ int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stre
   }
   CUtensorMap mk, mv;
   const long long rows = (long long)p.n_pages * p.kv_heads * p.page_size;
-  if (!group_map<HD>(&mk, p.k_pages, rows) || !group_map<HD>(&mv, p.v_pages, rows))
+  constexpr CUtensorMapSwizzle SWIZZLE = HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
+  if (!group_map(&mk, p.k_pages, rows, HD, SWIZZLE) || !group_map(&mv, p.v_pages, rows, HD, SWIZZLE))
     GB_FAIL(GB_ERR_CUDA, "kv8_attention: cuTensorMapEncodeTiled failed (%lld rows of %d)", rows, HD);
   const int parts = key_parts(tiles * p.kv_heads, 148 * C::CTAS, (keys + C::CK - 1) / C::CK, C::NW);
   return launch_parts(kv8_attention_mma_kernel<HD, NB>, p, parts, tiles, 32 * C::NW, SMEM, stream, mk, mv);

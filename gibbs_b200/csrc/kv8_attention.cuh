@@ -49,6 +49,16 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) { return ((((w & 0x7f7
 // log2 of a power of two (the sign does not matter)
 __device__ __forceinline__ float log2_of(float scale) { return (float)((int)((__float_as_uint(scale) >> 23) & 0xffu) - 127); }
 
+// The pool of pages [rows, hd] as a tensor map whose copies are groups of sixteen rows.
+static bool group_map(CUtensorMap* map, const void* pages, long long rows, int hd, CUtensorMapSwizzle swizzle) {
+  const TensorMapFn fn = tensor_map_fn();
+  if (!fn) return false;
+  const cuuint64_t dims[2] = {(cuuint64_t)hd, (cuuint64_t)rows}, strides[1] = {(cuuint64_t)hd};
+  const cuuint32_t box[2] = {(cuuint32_t)hd, 16}, step[2] = {1, 1};
+  return fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(pages), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 // Launches `kernel` over the tiles, their kv heads and parts (x in this order, parts fastest: the tiles with the most keys of
 // every head start first), a tile's parts as a cluster.
 template <typename K, typename... Maps>

@@ -4,9 +4,9 @@
 // A CTA takes 256 consecutive (token, head of a kv head's group) rows of one request, as two tiles of 128, and walks their
 // visible keys in tiles of 128:
 //
-//   warps 8-11   bring K_j and V_j: sixteen bytes a lane from the pages (asked for one item ahead), e4m3 to f16, which holds
-//                every number exactly, into a ring of swizzled tiles; K_j brings the scales of its pages along
-//   warp 12      one thread issues S = Q K_j^T for both row tiles and, when a tile's weights are there, O += P V_j and the next S
+//   warps 8-10   bring K_j and V_j: from the pages by cp.async, some items ahead, then e4m3 to f16, which holds every number exactly,
+//                into a ring of swizzled tiles; K_j brings the scales of its pages along
+//   warp 11      one thread issues S = Q K_j^T for both row tiles and, when a tile's weights are there, O += P V_j and the next S
 //   warps 0-7    a thread has a row: reads S from tensor memory, scales, masks, running maximum and sum in 32 bits, writes the
 //                weights in f16 over S in tensor memory, from where they are the A operand of the second product
 //
@@ -29,17 +29,23 @@ using namespace kv8;
 using namespace sm100;
 
 constexpr int ROWS = 128, KEYS = 128, GROUPS = KEYS / 16;
-constexpr int THREADS = 416;                                  // 8 softmax warps, 4 that convert, 1 that issues
+constexpr int THREADS = 384;                                  // 8 softmax warps, 3 that convert, 1 that issues: 168 registers a thread
+constexpr int CONVERTERS = 96;
 constexpr int META = 4;                                       // tiles whose scales are kept
 
 template <int HD> struct Cfg {
   static constexpr int SUB = HD / 64;                         // 64-column sub-tiles
-  static constexpr int RING = 4;                              // f16 tiles of K or V
+  // Tensor memory has room for weights of their own beside S and O of two row tiles at head_dim 64: the next S then goes out as soon
+  // as S has been read.  At 128 the weights lie over S, and the next S goes out behind the product that reads them.
+  static constexpr bool APART = HD == 64;
+  static constexpr int RING = APART ? 4 : 3;                  // f16 tiles of K or V
+  static constexpr int STAGES = APART ? 4 : 3;                // tiles of K or V as they come
+  static constexpr int RAW_TILE = KEYS * HD;
   static constexpr int Q_TILE = ROWS * HD * 2, KV_TILE = KEYS * HD * 2;
   static constexpr int NAN_BYTES = META * KEYS * HD / 8;      // which values of a tile are NaN, a bit each
   static constexpr int SHARE = 2 * ROWS * HD * 4 + 2 * ROWS * 8;
   static constexpr int OPERANDS = 2 * Q_TILE + RING * KV_TILE;
-  static constexpr int SMEM = OPERANDS + NAN_BYTES + 1024;
+  static constexpr int SMEM = OPERANDS + STAGES * RAW_TILE + NAN_BYTES + 1024;
   static_assert(SHARE <= OPERANDS, "a share of O and its (m, l) fit over the operands");
   static_assert(SMEM <= 227 * 1024, "shared memory");
 };
@@ -56,6 +62,18 @@ __device__ __forceinline__ void umma_f16_ta(uint32_t tmem_d, uint32_t tmem_a, ui
       : "memory");
 }
 
+__device__ __forceinline__ void tmem_st_16_issue(uint32_t taddr, const uint32_t* v) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};"
+      ::"r"(taddr), "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+        "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
+      : "memory");
+}
+__device__ __forceinline__ void tmem_st_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+__device__ __forceinline__ void cp_async_16(uint32_t smem, const void* gmem, int n) {            // n = 0: filled with zeros
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(smem), "l"(gmem), "r"(n) : "memory");
+}
 __device__ __forceinline__ uint64_t pk2(float a, float b) {
   uint64_t r;
   asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(a), "f"(b));
@@ -88,7 +106,8 @@ template <int HD>
 __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const Attn p) {
   using C = Cfg<HD>;
   extern __shared__ uint8_t smem_raw[];
-  __shared__ uint64_t q_full, kv_full[C::RING], kv_empty[C::RING], s_full[2], p_full[2], o_full[2];
+  __shared__ uint64_t q_full, kv_full[C::RING], kv_empty[C::RING], s_full[2], s_free[2], p_full[2][2], o_done[2];
+  __shared__ int marks[META];                                 // whether any page of the tile has NaN among its values
   __shared__ float4 meta[META][GROUPS];                       // of a group of sixteen keys: |scale of K|, log2 and inverse of V's scale,
                                                               // 1 where V's page holds NaN
   __shared__ uint32_t tmem_slot;
@@ -96,7 +115,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   uint8_t* base = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
   uint8_t* sq = base;                                         // [2][SUB][128 rows][128 B]
   uint8_t* skv = sq + 2 * C::Q_TILE;                          // [RING][SUB][128 keys][128 B]
-  uint32_t* snan = reinterpret_cast<uint32_t*>(skv + C::RING * C::KV_TILE);          // [META][128 keys][HD / 32]
+  uint8_t* sraw = skv + C::RING * C::KV_TILE;                 // [STAGES][128 keys][HD]
+  uint32_t* snan = reinterpret_cast<uint32_t*>(sraw + C::STAGES * C::RAW_TILE);          // [META][128 keys][HD / 32]
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = p.heads / p.kv_heads, tpt = ROWS / group;  // tokens of a row tile
   const int part = (int)blockIdx.x % p.parts, unit = (int)blockIdx.x / p.parts, kvh = unit % p.kv_heads;
@@ -130,18 +150,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   if (threadIdx.x == 0) {
     mbar_init(&q_full, 8);
     for (int s = 0; s < C::RING; ++s) {
-      mbar_init(&kv_full[s], 4);
+      mbar_init(&kv_full[s], CONVERTERS / 32);
       mbar_init(&kv_empty[s], 1);
     }
     for (int x = 0; x < 2; ++x) {
       mbar_init(&s_full[x], 1);
-      mbar_init(&p_full[x], 4);
-      mbar_init(&o_full[x], 1);
+      mbar_init(&s_free[x], 4);
+      mbar_init(&p_full[x][0], 4);                             // (a barrier for each half of a tile's weights: a warp may be a half ahead)
+      mbar_init(&p_full[x][1], 4);
+      mbar_init(&o_done[x], 1);
     }
     abort_flag = 0;
     fence_barrier_init();
   }
-  if (warp == 12) {
+  if (warp == 11) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
   }
@@ -150,107 +172,151 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   tc_fence_after();
   const uint32_t tmem = tmem_slot;
   const uint32_t tmem_s[2] = {tmem, tmem + KEYS}, tmem_o[2] = {tmem + 2 * KEYS, tmem + 2 * KEYS + HD};
+  const uint32_t tmem_p[2] = {C::APART ? tmem + 2 * KEYS + 2 * HD : tmem, C::APART ? tmem + 2 * KEYS + 2 * HD + KEYS / 2 : tmem + KEYS};
   pdl_wait();
 
-  if (warp >= 8 && warp < 12) {
+  if (warp >= 8 && warp < 11) {
     // ---- K and V: pages -> f16 tiles ----
-    constexpr int PIECES = HD / 16, ROWS_STEP = 128 / PIECES, STEPS = KEYS / ROWS_STEP;      // 16-byte pieces of a row
-    const int tid = threadIdx.x - 256, piece = tid % PIECES, row_in = tid / PIECES;
+    // Item 2 j is K of the CTA's key tile j, item 2 j + 1 its V.  A warp has whole groups of sixteen keys, which lie in one page and
+    // there one behind the other: one address for a group, and the rest are constants.  A lane copies the very pieces that it will
+    // convert (cp.async, STAGES items ahead), so nothing but its own copies is waited for.  (By TMA, a copy a group, the copies of an
+    // item took a warp longer to issue than its conversion.)
+    constexpr int PIECES = HD / 16, PER = 16 * PIECES / 32;   // 16-byte pieces of a row; of a group, for a lane
+    constexpr int ROWS_STEP = 32 / PIECES;                    // rows from one of a lane's pieces to the next
+    constexpr int MINE = (GROUPS + CONVERTERS / 32 - 1) / (CONVERTERS / 32);
+    const int w0 = warp - 8, piece = lane % PIECES, row_in = lane / PIECES;      // groups w0, w0 + 3, w0 + 6 < 8
     const int* bt = p.block_table + (size_t)r * p.bt_stride;
-    // lane i < 8: page of group i of a tile, -1 where nothing of it is visible
-    auto page_of = [&](int t) {
-      const int j = t * KEYS + lane * 16;
-      if (lane >= GROUPS || t >= t_hi || j >= hi || j + 15 < lo) return -1;
-      const int page = bt[j >> p.page_shift];
+    // lane i < 8: page of group i of a tile, -1 where nothing of it is visible (and in the other lanes)
+    auto page_of = [&](int j) {
+      const int key = (t_lo + j) * KEYS + lane * 16;
+      if (lane >= GROUPS || j >= n || key >= hi || key + 15 < lo) return -1;
+      const int page = bt[key >> p.page_shift];
       if (page >= 0 && page < p.n_pages) return page;
       if (warp == 8) atomicExch(p.status, STATUS_BAD_PAGE_READ);
       return -1;
     };
-    // this lane's pieces of an item: of K (or V) of tile t, whose groups' pages the lanes hold
-    auto fetch = [&](const uint8_t* pages, int t, int page, uint4 (&w)[STEPS]) {
+    uint8_t* mine = sraw + lane * 16;
+    const size_t head = (size_t)kvh << p.page_shift;
+    // Asks for an item; what is not visible, or behind the context (which holds anything, and 0 * NaN is not 0), comes as zeros.
+    auto request = [&](int it, int page) {
+      if (it < 2 * n) {
+        const uint8_t* pool = ((it & 1) ? p.v_pages : p.k_pages) + lane * 16;
+        const int key0 = (t_lo + (it >> 1)) * KEYS;
+        const uint32_t dst = smem_u32(mine) + (uint32_t)((it % C::STAGES) * C::RAW_TILE);
 #pragma unroll
-      for (int i = 0; i < STEPS; ++i) {
-        const int row = row_in + i * ROWS_STEP, j = t * KEYS + row;
-        const int pg = __shfl_sync(0xffffffffu, page, row >> 4);
-        w[i] = make_uint4(0u, 0u, 0u, 0u);
-        if (pg >= 0 && j < hi)                                 // (rows behind the context hold anything: 0 * NaN is not 0)
-          w[i] = *reinterpret_cast<const uint4*>(pages + ((((size_t)pg * p.kv_heads + kvh) << p.page_shift) + (j & (p.page_size - 1))) * HD +
-                                                 piece * 16);
+        for (int y = 0; y < MINE; ++y) {
+          const int g = w0 + y * (CONVERTERS / 32), pg = __shfl_sync(0xffffffffu, page, g), key = key0 + 16 * g;
+          if (g >= GROUPS) continue;
+          const uint8_t* src = pool + (pg < 0 ? 0 : ((((size_t)pg * p.kv_heads) << p.page_shift) + head + (key & (p.page_size - 1))) * HD);
+          const int rows = pg < 0 ? 0 : hi - key - row_in;     // (positive: there)
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            cp_async_16(dst + (uint32_t)(g * 16 * HD + i * 512), src + i * 512, rows > i * ROWS_STEP ? 16 : 0);
+        }
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    };
+    float ks = 0.f, vs = 0.f, ks_next, vs_next;                // scales of this lane's group, in this tile and in the next
+    auto scales = [&](int page, float& k, float& v) {
+      k = v = 0.f;
+      if (page >= 0) {
+        k = p.k_scales[(size_t)page * p.kv_heads + kvh];
+        v = p.v_scales[(size_t)page * p.kv_heads + kvh];
       }
     };
-    int page = page_of(t_lo), page_next = page_of(t_lo + 1);
-    uint4 kw[STEPS], vw[STEPS];
-    float ks = 0.f, vs = 0.f;                                  // of this lane's group
-    auto scales = [&](int pg) {
-      ks = vs = 0.f;
-      if (pg >= 0) {
-        ks = p.k_scales[(size_t)pg * p.kv_heads + kvh];
-        vs = p.v_scales[(size_t)pg * p.kv_heads + kvh];
-      }
-    };
-    if (n > 0) {
-      fetch(p.k_pages, t_lo, page, kw);
-      scales(page);
-    }
+    // pages of tile j, j + 1, ... (a request goes out at most STAGES items, two tiles, ahead)
+    int pages[4] = {page_of(0), page_of(1), page_of(2), page_of(3)};
+#pragma unroll
+    for (int it = 0; it < C::STAGES; ++it) request(it, pages[it >> 1]);
+    scales(pages[0], ks, vs);
     for (int j = 0; j < n; ++j) {
-      fetch(p.v_pages, t_lo + j, page, vw);
+      scales(pages[1], ks_next, vs_next);                      // asked for a tile ahead
       const uint32_t marked = __ballot_sync(0xffffffffu, lane < GROUPS && vs < 0.f);
+      if (warp == 8 && lane == 0) marks[j % META] = marked != 0u;
       if (warp == 8 && lane < GROUPS)
         meta[j % META][lane] = ks == 0.f ? make_float4(0.f, -INFINITY, 0.f, 0.f)
                                          : make_float4(fabsf(ks), log2_of(vs), inverse(vs), vs < 0.f ? 1.f : 0.f);
       if (marked) {
-        // which values of the tile are NaN: rows that see their key have NaN there, and the products get 0 instead
+        // Which values of the tile are NaN: rows that see their key have NaN there (the products get 0 instead).  The rows' threads
+        // look at it with the scores, which may be ahead of the values: it goes out with the keys.
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 2) : "memory");
         uint16_t* at = reinterpret_cast<uint16_t*>(snan) + (size_t)(j % META) * KEYS * PIECES;
+#pragma unroll 1
+        for (int g = w0; g < GROUPS; g += CONVERTERS / 32)
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          uint32_t* w = reinterpret_cast<uint32_t*>(&vw[i]);
-          uint32_t which = 0u;
+          for (int i = 0; i < PER; ++i) {
+            const uint4 v = *reinterpret_cast<const uint4*>(mine + (size_t)((2 * j + 1) % C::STAGES) * C::RAW_TILE + g * 16 * HD + i * 512);
+            const uint32_t w[4] = {nan_bytes(v.x), nan_bytes(v.y), nan_bytes(v.z), nan_bytes(v.w)};
+            uint32_t which = 0u;
 #pragma unroll
-          for (int x = 0; x < 4; ++x) {
-            const uint32_t bad = nan_bytes(w[x]);
-            w[x] &= ~bad;
-            which |= ((bad & 1u) | ((bad >> 7) & 2u) | ((bad >> 14) & 4u) | ((bad >> 21) & 8u)) << (4 * x);
+            for (int x = 0; x < 4; ++x) which |= ((w[x] & 1u) | ((w[x] >> 7) & 2u) | ((w[x] >> 14) & 4u) | ((w[x] >> 21) & 8u)) << (4 * x);
+            at[(16 * g + row_in + i * ROWS_STEP) * PIECES + piece] = (uint16_t)which;
           }
-          at[(row_in + i * ROWS_STEP) * PIECES + piece] = (uint16_t)which;
-        }
       }
-#pragma unroll
+#pragma unroll 1
       for (int kv = 0; kv < 2; ++kv) {
         const int it = 2 * j + kv, s = it % C::RING;
+        asm volatile("cp.async.wait_group %0;" ::"n"(C::STAGES - 1) : "memory");
+        uint4 w[MINE][PER];
+#pragma unroll
+        for (int y = 0; y < MINE; ++y)
+#pragma unroll
+          for (int i = 0; i < PER; ++i)
+            w[y][i] = *reinterpret_cast<const uint4*>(mine + (size_t)(it % C::STAGES) * C::RAW_TILE + min(w0 + y * (CONVERTERS / 32), GROUPS - 1) * 16 * HD +
+                                                      i * 512);
         if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[s], ((it / C::RING) & 1) ^ 1) && !abort_flag)) {
           abort_flag = 1;
           if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT);
           break;
         }
-        uint8_t* dst = skv + (size_t)s * C::KV_TILE;
+        if (marked && kv == 1) {
 #pragma unroll
-        for (int i = 0; i < STEPS; ++i) {
-          const int row = row_in + i * ROWS_STEP;
-          const uint4 w = kv == 0 ? kw[i] : vw[i];
-          uint4 a, b;
-          to_f16(w.x, a.x, a.y);
-          to_f16(w.y, a.z, a.w);
-          to_f16(w.z, b.x, b.y);
-          to_f16(w.w, b.z, b.w);
-          // chunks 2 piece, 2 piece + 1 of the row's HD / 8; a sub-tile has 8
-          uint8_t* at = dst + (size_t)(piece / 4) * KEYS * 128 + (size_t)row * 128;
-          const int c = (2 * piece) & 7;
-          *reinterpret_cast<uint4*>(at + ((c ^ (row & 7)) << 4)) = a;
-          *reinterpret_cast<uint4*>(at + (((c + 1) ^ (row & 7)) << 4)) = b;
+          for (int y = 0; y < MINE; ++y)
+#pragma unroll
+            for (int i = 0; i < PER; ++i) {
+              w[y][i].x &= ~nan_bytes(w[y][i].x);
+              w[y][i].y &= ~nan_bytes(w[y][i].y);
+              w[y][i].z &= ~nan_bytes(w[y][i].z);
+              w[y][i].w &= ~nan_bytes(w[y][i].w);
+            }
+        }
+        // chunks 2 piece, 2 piece + 1 of the row's HD / 8; a sub-tile has 8
+        uint8_t* dst = skv + (size_t)s * C::KV_TILE + (size_t)(piece / 4) * KEYS * 128 + row_in * 128;
+        constexpr int TURNS = 8 / ROWS_STEP > 1 ? 8 / ROWS_STEP : 1;      // of a lane's rows: different places in the swizzle
+        int c0[TURNS];
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) c0[i] = ((((2 * piece) & 7) ^ ((row_in + i * ROWS_STEP) & 7)) << 4);
+#pragma unroll
+        for (int y = 0; y < MINE; ++y) {
+          const int g = w0 + y * (CONVERTERS / 32);
+          if (g >= GROUPS) continue;
+#pragma unroll
+          for (int i = 0; i < PER; ++i) {
+            uint4 a, b;
+            to_f16(w[y][i].x, a.x, a.y);
+            to_f16(w[y][i].y, a.z, a.w);
+            to_f16(w[y][i].z, b.x, b.y);
+            to_f16(w[y][i].w, b.z, b.w);
+            uint8_t* at = dst + g * 16 * 128 + i * ROWS_STEP * 128;
+            *reinterpret_cast<uint4*>(at + c0[i % TURNS]) = a;
+            *reinterpret_cast<uint4*>(at + (c0[i % TURNS] ^ 16)) = b;
+          }
         }
         fence_proxy_async();                                   // read by the tensor core (async proxy)
         __syncwarp();
         if (lane == 0) mbar_arrive(&kv_full[s]);
-        if (kv == 0 && j + 1 < n) {                            // the next tile's keys are asked for while this one's values are converted
-          page = page_next;
-          fetch(p.k_pages, t_lo + j + 1, page, kw);
-          scales(page);
-          page_next = page_of(t_lo + j + 2);
-        }
+        request(it + C::STAGES, ((it + C::STAGES) >> 1) == j + 1 ? pages[1] : pages[2]);        // (into the stage that has been read)
       }
       if (abort_flag) break;
+      ks = ks_next;
+      vs = vs_next;
+      pages[0] = pages[1];
+      pages[1] = pages[2];
+      pages[2] = pages[3];
+      pages[3] = page_of(j + 4);
     }
-  } else if (warp == 12) {
+    asm volatile("cp.async.wait_group 0;" ::: "memory");
+  } else if (warp == 11) {
     // ---- the products ----
     if (elect_one()) {
       constexpr uint32_t idesc_s = idesc_f16(ROWS, KEYS), idesc_o = idesc_f16_b_mn(ROWS, HD);
@@ -270,6 +336,24 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
         tc_fence_after();
         return ok;
       };
+      // O += P V_j for a row tile, in two halves of the keys as the weights come; kv_ready(V_j) has been seen
+      auto issue_o = [&](int x, int j) {
+        const uint8_t* vt = skv + (size_t)((2 * j + 1) % C::RING) * C::KV_TILE;
+#pragma unroll
+        for (int k = 0; k < KEYS / 16; ++k) {
+          if (k % (KEYS / 32) == 0) {
+            if (!mbar_wait(&p_full[x][k / (KEYS / 32)], j & 1)) return false;
+            tc_fence_after();
+          }
+          // 16 keys = two 8-row groups of 1024 bytes further in V; a second 64-column block of head_dim (128) lies one sub-tile
+          // further, which the descriptor's leading offset says
+          uint64_t db = smem_desc_sw128(vt + (size_t)k * 16 * 128);
+          if (C::SUB > 1) db = (db & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)((KEYS * 128) >> 4) << 16);
+          umma_f16_ta(tmem_o[x], tmem_p[x] + 8 * k, db, idesc_o, (uint32_t)((j | k) != 0));
+        }
+        if (C::APART || j + 1 == n_x[x]) umma_commit(&o_done[x]);
+        return true;
+      };
       bool ok = mbar_wait(&q_full, 0);
       tc_fence_after();
       if (ok && n > 0) {
@@ -278,34 +362,47 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
           if (n_x[x] > 0) issue_s(x, 0);
         umma_commit(&kv_empty[0]);
       }
-      for (int j = 0; j < n && ok && !abort_flag; ++j) {
-        ok = kv_ready(2 * j + 1);
-        if (!ok) break;
-        const uint8_t* vt = skv + (size_t)((2 * j + 1) % C::RING) * C::KV_TILE;
-        bool next = false;
-        for (int x = 0; x < 2 && ok; ++x) {
-          if (j >= n_x[x]) continue;
-          ok = mbar_wait(&p_full[x], j & 1);
-          if (!ok) break;
-          tc_fence_after();
-#pragma unroll
-          for (int k = 0; k < KEYS / 16; ++k) {
-            // 16 keys = two 8-row groups of 1024 bytes further in V; a second 64-column block of head_dim (128) lies one sub-tile
-            // further, which the descriptor's leading offset says
-            uint64_t db = smem_desc_sw128(vt + (size_t)k * 16 * 128);
-            if (C::SUB > 1) db = (db & ~((uint64_t)0x3FFF << 16)) | ((uint64_t)((KEYS * 128) >> 4) << 16);
-            umma_f16_ta(tmem_o[x], tmem_s[x] + 8 * k, db, idesc_o, (uint32_t)((j | k) != 0));
+      if (C::APART) {
+        // The row tiles run half a tile apart, and so do the steps here: S of the first, the product of the second's tile before, ...
+        // Step j: S_0(j + 1), O_1(j - 1), S_1(j + 1), O_0(j).  K_{j+1} is done with behind S_1(j + 1), V_{j-1} behind O_1(j - 1).
+        for (int j = 0; j <= n && ok && !abort_flag; ++j) {
+          const bool more = j + 1 < n;
+          if (more) ok = kv_ready(2 * j + 2);
+          if (ok && j + 1 < n_x[0]) {
+            ok = mbar_wait(&s_free[0], j & 1);
+            tc_fence_after();
+            if (ok) issue_s(0, j + 1);
           }
-          if (j + 1 == n_x[x]) umma_commit(&o_full[x]);
-          if (j + 1 < n_x[x]) {
-            if (!next) ok = kv_ready(2 * j + 2);
-            if (!ok) break;
-            next = true;
-            issue_s(x, j + 1);                                 // (behind P V_j in the tensor pipe, which reads the weights over S)
+          if (ok && j > 0) {
+            if (j - 1 < n_x[1]) ok = issue_o(1, j - 1);
+            umma_commit(&kv_empty[(2 * j - 1) % C::RING]);
           }
+          if (ok && j + 1 < n_x[1]) {
+            ok = mbar_wait(&s_free[1], j & 1);
+            tc_fence_after();
+            if (ok) issue_s(1, j + 1);
+          }
+          if (ok && more) umma_commit(&kv_empty[(2 * j + 2) % C::RING]);
+          if (ok && j < n) ok = kv_ready(2 * j + 1);
+          if (ok && j < n_x[0]) ok = issue_o(0, j);
         }
-        umma_commit(&kv_empty[(2 * j + 1) % C::RING]);
-        if (next) umma_commit(&kv_empty[(2 * j + 2) % C::RING]);
+      } else {
+        for (int j = 0; j < n && ok && !abort_flag; ++j) {
+          ok = kv_ready(2 * j + 1);
+          bool next = false;
+          for (int x = 0; x < 2 && ok; ++x) {
+            if (j >= n_x[x]) continue;
+            ok = issue_o(x, j);
+            if (ok && j + 1 < n_x[x]) {
+              if (!next) ok = kv_ready(2 * j + 2);
+              if (!ok) break;
+              next = true;
+              issue_s(x, j + 1);                               // (behind O_j in the tensor pipe, which reads the weights over S)
+            }
+          }
+          umma_commit(&kv_empty[(2 * j + 1) % C::RING]);
+          if (next) umma_commit(&kv_empty[(2 * j + 2) % C::RING]);
+        }
       }
       if (!ok) {
         abort_flag = 1;
@@ -354,12 +451,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
       __syncwarp();
       if (lane == 0) mbar_arrive(&q_full);
     }
-    float m = -INFINITY, l = 0.f;
+    float m = -INFINITY, l = 0.f;                              // the maximum in use and the sum
     uint32_t poison[HD / 32];                                  // columns that are NaN in this row
 #pragma unroll
     for (int i = 0; i < HD / 32; ++i) poison[i] = 0u;
     bool alive = true;
-    for (int j = 0; j < n_x[x]; ++j) {
+    const uint32_t tmem_x = x ? tmem_s[1] : tmem_s[0], tmem_ox = x ? tmem_o[1] : tmem_o[0], tmem_px = x ? tmem_p[1] : tmem_p[0];
+    const int n_mine = x ? n_x[1] : n_x[0];
+    for (int j = 0; j < n_mine; ++j) {
       if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1) && !abort_flag)) {
         abort_flag = 1;
         if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT + 2);
@@ -373,35 +472,34 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
       const int hi_c = valid ? pos - col0 : -1, lo_c = (p.window > 0 ? pos - p.window + 1 : 0) - col0;     // columns the row sees
       const bool none = hi_c < lo_c;
       const unsigned span = none ? 0u : (unsigned)(hi_c - lo_c);
-      // S is read twice, 64 columns at a time: once for the maximum, once for the weights (128 columns and their weights would not
-      // fit the 128 registers that a thread of thirteen warps has)
-      float v[64];
-      auto load = [&](int c) {
-        tmem_ld_32_issue(tmem_s[x] + lane_off + (uint32_t)c, v);
-        tmem_ld_32_issue(tmem_s[x] + lane_off + (uint32_t)(c + 32), v + 32);
-        tmem_ld_wait_n<64>(v);
-        if (!full) {
+      // the whole row of S into registers: the loads on their way together, one wait
+      float v[KEYS];
 #pragma unroll
-          for (int i = 0; i < 64; ++i) v[i] = (!none && (unsigned)(c + i - lo_c) <= span) ? v[i] : -INFINITY;
-        }
-      };
+      for (int c = 0; c < KEYS; c += 32) tmem_ld_32_issue(tmem_x + lane_off + (uint32_t)c, v + c);
+      tmem_ld_wait_n<KEYS>(v);
+      if (C::APART) {                                          // the next S may come
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&s_free[x]);
+      }
+      if (!full) {
+#pragma unroll
+        for (int i = 0; i < KEYS; ++i) v[i] = (!none && (unsigned)(i - lo_c) <= span) ? v[i] : -INFINITY;
+      }
       // the largest x = score + log2(scale of V) of the row
       float top = -INFINITY;
 #pragma unroll
-      for (int c = 0; c < KEYS; c += 64) {
-        load(c);
-#pragma unroll
-        for (int g = 0; g < 4; ++g) {
-          float a = fmaxf(v[16 * g], v[16 * g + 1]), b = fmaxf(v[16 * g + 2], v[16 * g + 3]);
-#pragma unroll
-          for (int i = 4; i < 16; i += 4) {
-            a = fmaxf(a, fmaxf(v[16 * g + i], v[16 * g + i + 1]));
-            b = fmaxf(b, fmaxf(v[16 * g + i + 2], v[16 * g + i + 3]));
-          }
-          const float2 sc = *reinterpret_cast<const float2*>(&mt[c / 16 + g]);
-          // (a factor that underflowed would make NaN of a masked column's -inf)
-          top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(factor * sc.x, 1.2e-38f), sc.y));
-        }
+      for (int g = 0; g < GROUPS; ++g) {
+        const float* u = v + 16 * g;
+        float a = fmaxf(fmaxf(u[0], u[1]), u[2]), b = fmaxf(fmaxf(u[3], u[4]), u[5]);
+        a = fmaxf(fmaxf(a, u[6]), u[7]);
+        b = fmaxf(fmaxf(b, u[8]), u[9]);
+        a = fmaxf(fmaxf(a, u[10]), u[11]);
+        b = fmaxf(fmaxf(b, u[12]), u[13]);
+        a = fmaxf(fmaxf(a, u[14]), u[15]);
+        const float2 sc = *reinterpret_cast<const float2*>(&mt[g]);
+        // (a factor that underflowed would make NaN of a masked column's -inf)
+        top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(factor * sc.x, 1.2e-38f), sc.y));
       }
       // the maximum in use follows only when it would fall behind by more than 2^3: a weight stays below 2^15
       float corr = 1.f;
@@ -410,64 +508,70 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
         m = top;
         l *= corr;
       }
-      if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
-        // (S_j was issued behind P V_{j-1}: O stands still)
-#pragma unroll 1
-        for (int c0 = 0; c0 < HD; c0 += 32) {
-          float* o = v;
-          tmem_ld_32(tmem_o[x] + lane_off + (uint32_t)c0, o);
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] *= corr;
-          tmem_st_32(tmem_o[x] + lane_off + (uint32_t)c0, o);
-        }
-      }
       const float off = 12.f - (m == -INFINITY ? 0.f : m);
-#pragma unroll
-      for (int c0 = 0; c0 < KEYS; c0 += 64) {
-        load(c0);                                              // (the weights of columns up to c0 lie in columns up to c0 / 2)
-#pragma unroll
-        for (int h32 = 0; h32 < 2; ++h32) {
-          uint32_t packed[16];
-#pragma unroll
-          for (int y = 0; y < 2; ++y) {
-            const int g = 2 * h32 + y;                         // of the 64 columns
-            const float4 sc = mt[c0 / 16 + g];
-            const float f = fmaxf(factor * sc.x, 1.2e-38f), c = sc.y + off;
-            const uint64_t f2 = pk2(f, f), c2 = pk2(c, c);
-            uint64_t sum[2] = {0ull, 0ull};
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              float x0, x1, e0, e1;
-              upk2(fma2(pk2(v[16 * g + i], v[16 * g + i + 1]), f2, c2), x0, x1);
-              e0 = ex2(x0);
-              e1 = ex2(x1);
-              sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pk2(e0, e1));
-              packed[8 * y + i / 2] = pack_f16(e0, e1);
-            }
-            float a, b;
-            upk2(add2(sum[0], sum[1]), a, b);
-            l = fmaf(a + b, sc.z, l);
-            if (sc.w != 0.f) {
-              // values of this page that are NaN, for the keys that the row sees
-              const uint32_t* at = snan + ((size_t)(j % META) * KEYS + c0 + 16 * g) * (HD / 32);
+      if (C::APART && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[x], (j - 1) & 1) && !abort_flag)) {
+        abort_flag = 1;                                        // (P and O of the tile before are read by its product until then)
+        if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT + 3);
+        alive = false;
+        break;
+      }
+      if (C::APART) tc_fence_after();
+      if (j > 0 && __any_sync(0xffffffffu, corr != 1.f)) {
+        // (weights over S: S_j was issued behind P V_{j-1}, so O stands still here as well)
 #pragma unroll 1
-              for (int i = 0; i < 16; ++i) {
-                const int key = col0 + c0 + 16 * g + i;
-                if (valid && key <= pos && (p.window <= 0 || key + p.window > pos)) {
+        for (int c0 = 0; c0 < HD; c0 += 16) {
+          float o[16];
+          tmem_ld_16(tmem_ox + lane_off + (uint32_t)c0, o);
 #pragma unroll
-                  for (int w = 0; w < HD / 32; ++w) poison[w] |= at[i * (HD / 32) + w];
-                }
-              }
-            }
-          }
-          tmem_st_16(tmem_s[x] + lane_off + (uint32_t)((c0 + 32 * h32) / 2), reinterpret_cast<const float*>(packed));
+          for (int i = 0; i < 16; ++i) o[i] *= corr;
+          tmem_st_16(tmem_ox + lane_off + (uint32_t)c0, o);
         }
       }
-      tc_fence_before();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t packed[32];
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const float* u = v + 64 * half + 16 * g;
+          const float4 sc = mt[4 * half + g];
+          const float f = fmaxf(factor * sc.x, 1.2e-38f), d = sc.y + off;
+          const uint64_t f2 = pk2(f, f), d2 = pk2(d, d);
+          uint64_t sum[2] = {0ull, 0ull};
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) {
+            float x0, x1;
+            upk2(fma2(pk2(u[i], u[i + 1]), f2, d2), x0, x1);
+            const float e0 = ex2(x0), e1 = ex2(x1);
+            sum[(i >> 1) & 1] = add2(sum[(i >> 1) & 1], pk2(e0, e1));
+            packed[8 * g + i / 2] = pack_f16(e0, e1);
+          }
+          float a, b;
+          upk2(add2(sum[0], sum[1]), a, b);
+          l = fmaf(a + b, sc.z, l);
+        }
+        tmem_st_16_issue(tmem_px + lane_off + (uint32_t)(32 * half), packed);
+        tmem_st_16_issue(tmem_px + lane_off + (uint32_t)(32 * half + 16), packed + 16);
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (half == 0 && lane == 0) mbar_arrive(&p_full[x][0]);
+      }
+      if (marks[j % META]) {
+        // values of the tile's pages that are NaN, for the keys that the row sees
+        const uint32_t* at = snan + (size_t)(j % META) * KEYS * (HD / 32);
+#pragma unroll 1
+        for (int i = 0; i < KEYS; ++i) {
+          const int key = col0 + i;
+          if (mt[i / 16].w != 0.f && valid && key <= pos && (p.window <= 0 || key + p.window > pos)) {
+#pragma unroll
+            for (int w = 0; w < HD / 32; ++w) poison[w] |= at[i * (HD / 32) + w];
+          }
+        }
+      }
       __syncwarp();
-      if (lane == 0) mbar_arrive(&p_full[x]);
+      if (lane == 0) mbar_arrive(&p_full[x][1]);
     }
-    if (alive && n_x[x] > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_full[x], 0))) {
+    if (alive && n_mine > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[x], C::APART ? (n_mine - 1) & 1 : 0))) {
       abort_flag = 1;
       if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT + 3);
       alive = false;
@@ -480,7 +584,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
 #pragma unroll 1
     for (int c0 = 0; c0 < HD; c0 += 32) {
       float o[32];
-      if (n_x[x] > 0) tmem_ld_32(tmem_o[x] + lane_off + (uint32_t)c0, o);
+      if (n_mine > 0) tmem_ld_32(tmem_ox + lane_off + (uint32_t)c0, o);
       else
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0.f;
@@ -548,7 +652,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   pdl_trigger();
   tc_fence_before();
   __syncthreads();
-  if (warp == 12) tmem_dealloc(tmem_slot, 512);
+  if (warp == 11) tmem_dealloc(tmem_slot, 512);
 }
 
 template <int HD>
