@@ -155,6 +155,299 @@ int launch_any(const Store& p, long long segments, cudaStream_t stream) {
   return GB_OK;
 }
 
+// ---------------------------------------------------------------- heads of 64 or 128, the rotation over the whole head (or none)
+// HD / 8 threads share a row, eight neighbouring values each: sixteen bytes of bfloat16 in, eight bytes of numbers out.  The sum of
+// squares and the rotation's partner (HD / 2 further) come from the neighbours by shuffles.
+template <typename T>
+__device__ __forceinline__ void load8(const Store& p, int row, int col, float* v) {
+  if (p.splits > 0) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = 0.f;
+    const float* src = p.part + (size_t)row * p.ld + col;
+    for (int s = 0; s < p.splits; ++s, src += p.part_stride) {
+      const float4 a = ldcg_now(reinterpret_cast<const float4*>(src)), b = ldcg_now(reinterpret_cast<const float4*>(src) + 1);
+      v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
+      v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      if (p.part_bias) v[e] += p.part_bias[col + e];
+      v[e] = to_f32(from_f32<T>(v[e]));                        // rounded where the product's own sum would have been
+    }
+    return;
+  }
+  const T* src = reinterpret_cast<const T*>(p.rows) + (size_t)row * p.ld + col;
+  if constexpr (sizeof(T) == 2) {
+    const uint4 raw = *reinterpret_cast<const uint4*>(src);
+    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v[2 * e] = __uint_as_float(w[e] << 16);
+      v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
+    }
+  } else {
+    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store8(T* dst, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
+      w[e] = *reinterpret_cast<const uint32_t*>(&b);
+    }
+    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
+  } else {
+    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
+    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
+  }
+}
+// Norm (gain: this thread's eight, or none) and rotation (cs: the row's HD / 2 pairs of cos and sin, or null) of a row whose eight
+// values v this thread has; `sub` is the thread's place in the row.  All lanes of the warp take part.
+template <int HD>
+__device__ __forceinline__ void norm_rotate(float* v, const float* gain, bool norm, float eps, const float2* cs, int sub) {
+  constexpr int TPR = HD / 8;
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+#pragma unroll
+  for (int o = TPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+  if (norm) {
+    const float scale = 1.0f / sqrtf(ss * (1.f / HD) + eps);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = v[e] * scale * gain[e];
+  }
+  float w[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) w[e] = __shfl_xor_sync(0xffffffffu, v[e], TPR / 2);
+  if (cs != nullptr) {
+    const bool lower = sub < TPR / 2;
+    const float4* c4 = reinterpret_cast<const float4*>(cs + (lower ? sub : sub - TPR / 2) * 8);
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const float4 t = c4[e / 2];                              // cos, sin of two pairs
+      v[e] = lower ? v[e] * t.x - w[e] * t.y : w[e] * t.y + v[e] * t.x;
+      v[e + 1] = lower ? v[e + 1] * t.z - w[e + 1] * t.w : w[e + 1] * t.w + v[e + 1] * t.z;
+    }
+  }
+}
+__device__ __forceinline__ void magnitude8(const float* v, float& amax, bool& bad) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    if (holdable(v[e])) amax = fmaxf(amax, fabsf(v[e]));
+    else bad = true;
+  }
+}
+
+// Steps in which every request brings one token: a row is a unit, and 256 / HD of a block's 128 threads' rows make a warp's.  What
+// the step's metadata and the tables give (position, page, angles, gains) is worked out before the wait for the product in front.
+// Bound by the chain of trips: 4.3 us a call by itself, caches warm, at 8 tokens of 32 / 8 heads of 64.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) kv8_store_rows_kernel(const Store p) {
+  constexpr int TPR = HD / 8, SLOTS = 128 / TPR;
+  __shared__ __align__(16) float2 cs[HD / 2];
+  pdl_trigger();
+  const int r = blockIdx.y, sub = threadIdx.x % TPR, slot = (int)blockIdx.x * SLOTS + threadIdx.x / TPR;
+  const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
+  const bool active = slot < slots;
+  const bool is_q = slot < p.heads, is_k = !is_q && slot < p.heads + p.kv_heads;
+  const int pos = p.step.start_pos[r], row = p.step.q_start[r];
+  if (p.step.q_len[r] <= 0) return;                            // (the whole block)
+  int page = -1;
+  if (active && !is_q) page = p.block_table[(size_t)r * p.bt_stride + pos / p.page_size];
+  const int held = pos % p.page_size;                          // rows that the page holds already
+  if (p.rotary)
+    for (int j = threadIdx.x; j < HD / 2; j += 128) {
+      const float2 t = turn(pos, p.rotary[j]);
+      cs[j] = make_float2(t.x * p.rotary[HD / 2], t.y * p.rotary[HD / 2]);
+    }
+  const float* gain_at = is_q ? p.q_gain : is_k ? p.k_gain : nullptr;
+  const bool norm = active && gain_at != nullptr;
+  float gain[8];
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    gain[e] = norm ? gain_at[sub * 8 + e] : 1.f;
+    gb_pin(gain[e]);
+  }
+  gb_pin(page);
+  pdl_wait();
+  float v[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+  float was = 0.f;
+  const int kvh = active && !is_q ? (slot - p.heads) % p.kv_heads : 0;
+  const bool there = page >= 0 && page < p.n_pages;
+  float* scale_at = (is_k ? p.k_scales : p.v_scales) + (there ? (size_t)page * p.kv_heads + kvh : 0);
+  if (active) load8<T>(p, row, slot * HD + sub * 8, v);
+  if (there && held > 0) was = *scale_at;
+  __syncthreads();                                             // the angles
+  norm_rotate<HD>(v, gain, norm, p.eps, active && (is_q || is_k) && p.rotary ? cs : nullptr, sub);
+  float amax = 0.f;
+  bool bad = false;
+  magnitude8(v, amax, bad);
+#pragma unroll
+  for (int o = TPR / 2; o > 0; o >>= 1) {
+    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
+    bad |= __shfl_xor_sync(0xffffffffu, bad ? 1 : 0, o) != 0;
+  }
+  if (!active) return;
+  if (is_q) {
+    store8<T>(reinterpret_cast<T*>(p.q_out) + ((size_t)row * p.heads + slot) * HD + sub * 8, v);
+    return;
+  }
+  if (!there) {
+    if (sub == 0) atomicExch(p.status, STATUS_BAD_PAGE_WRITE);
+    return;
+  }
+  uint8_t* dst = (is_k ? p.k_pages : p.v_pages) + ((size_t)page * p.kv_heads + kvh) * p.page_size * HD + sub * 8;
+  const float now = fmaxf(fabsf(was), scale_for(amax)), inv = inverse(now);
+  if (held > 0 && fabsf(was) < now) {
+    const float ratio = fabsf(was) * inv;
+#pragma unroll 4
+    for (int i = 0; i < held; ++i) {
+      uint2* at = reinterpret_cast<uint2*>(dst + (size_t)i * HD);
+      *at = again8(*at, ratio);
+    }
+  }
+  *reinterpret_cast<uint2*>(dst + (size_t)held * HD) = pack8(v, inv);
+  if (sub == 0) *scale_at = (bad || signbit(was)) ? -now : now;
+}
+
+// Portions: a block has one page that a request writes to, and runs over a share of its heads.  A unit (a page's new rows of one
+// head) is held in registers by page_size / 16 warps, sixteen rows each, from the load to the store, so a row is read once; its
+// angles are worked out once a block into shared memory.
+template <typename T, int HD>
+__global__ void __launch_bounds__(256) kv8_store_pages_kernel(const Store p, int per_block) {
+  constexpr int TPR = HD / 8, RPP = 32 / TPR, PASSES = 16 / RPP;       // threads of a row, rows of a pass, passes of sixteen rows
+  extern __shared__ __align__(16) float2 cs_all[];                     // [new rows][HD / 2]
+  __shared__ float top_of[8];
+  __shared__ int bad_of[8];
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % TPR;
+  int seg = 0;
+  const int r = find_piece((int)blockIdx.x, p.step.n_requests, false, [&](int i) {
+    const int n = p.step.q_len[i], b = p.step.start_pos[i];
+    return n > 0 ? (b + n - 1) / p.page_size - b / p.page_size + 1 : 0;
+  }, seg);
+  if (r < 0) return;
+  const int before = p.step.start_pos[r], end = before + p.step.q_len[r];
+  const int block = before / p.page_size + seg, base = block * p.page_size;
+  const int from = max(before, base) - base, to = min(end, base + p.page_size) - base;      // new rows of the page
+  const int row0 = p.step.q_start[r] + base - before;                   // batch row of the page's row 0 (if it were new)
+  const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
+  const int wpu = p.page_size / 16, wu = warp % wpu, units = 8 / wpu;
+  int page = -1;
+  if (p.write) page = p.block_table[(size_t)r * p.bt_stride + block];
+  const bool there = page >= 0 && page < p.n_pages;
+  if (p.rotary)
+    for (int i = threadIdx.x; i < (to - from) * (HD / 2); i += 256) {
+      const float2 t = turn(base + from + i / (HD / 2), p.rotary[i % (HD / 2)]);
+      cs_all[i] = make_float2(t.x * p.rotary[HD / 2], t.y * p.rotary[HD / 2]);
+    }
+  pdl_wait();
+  __syncthreads();
+  if (p.write && !there && threadIdx.x == 0) atomicExch(p.status, STATUS_BAD_PAGE_WRITE);
+  const int slot_end = min(slots, (int)(blockIdx.y + 1) * per_block);
+  for (int slot0 = (int)blockIdx.y * per_block; slot0 < slot_end; slot0 += units) {
+    const int slot = slot0 + warp / wpu;
+    const bool is_q = slot < p.heads, is_k = !is_q && slot < p.heads + p.kv_heads;
+    const bool active = slot < slot_end && (is_q || there);
+    const int kvh = is_q ? 0 : (slot - p.heads) % p.kv_heads;
+    const float* gain_at = is_q ? p.q_gain : is_k ? p.k_gain : nullptr;
+    float v[PASSES][8];
+    bool mine[PASSES];
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int o = 16 * wu + i * RPP + lane / TPR;             // row of the page
+      mine[i] = active && o >= from && o < to;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
+      if (mine[i]) load8<T>(p, row0 + o, slot * HD + sub * 8, v[i]);
+    }
+    float gain[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) gain[e] = gain_at ? gain_at[sub * 8 + e] : 1.f;
+    float was = 0.f;
+    float* scale_at = (is_k ? p.k_scales : p.v_scales) + (there && !is_q ? (size_t)page * p.kv_heads + kvh : 0);
+    if (active && !is_q && from > 0) was = *scale_at;
+    float amax = 0.f;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int o = 16 * wu + i * RPP + lane / TPR;
+      norm_rotate<HD>(v[i], gain, gain_at != nullptr, p.eps,
+                      (is_q || is_k) && p.rotary ? cs_all + (size_t)(mine[i] ? o - from : 0) * (HD / 2) : nullptr, sub);
+      if (is_q) {
+        if (mine[i]) store8<T>(reinterpret_cast<T*>(p.q_out) + ((size_t)(row0 + o) * p.heads + slot) * HD + sub * 8, v[i]);
+      } else if (mine[i]) {
+        magnitude8(v[i], amax, bad);
+      }
+    }
+    // the page's largest magnitude, over the warps that hold it
+    amax = warp_max(amax);
+    bad = __any_sync(0xffffffffu, bad);
+    if (wpu > 1) {
+      if (lane == 0) {
+        top_of[warp] = amax;
+        bad_of[warp] = bad ? 1 : 0;
+      }
+      __syncthreads();
+      for (int i = 0; i < wpu; ++i) {
+        amax = fmaxf(amax, top_of[warp - wu + i]);
+        bad |= bad_of[warp - wu + i] != 0;
+      }
+      __syncthreads();
+    }
+    if (!active || is_q) continue;
+    uint8_t* dst = (is_k ? p.k_pages : p.v_pages) + ((size_t)page * p.kv_heads + kvh) * p.page_size * HD + sub * 8;
+    const float now = fmaxf(fabsf(was), scale_for(amax)), inv = inverse(now);
+    const bool grown = from > 0 && fabsf(was) < now;
+    const float ratio = fabsf(was) * inv;
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int o = 16 * wu + i * RPP + lane / TPR;
+      uint2* at = reinterpret_cast<uint2*>(dst + (size_t)o * HD);
+      if (mine[i]) *at = pack8(v[i], inv);
+      else if (grown && o < from) *at = again8(*at, ratio);
+    }
+    // (every warp of the unit has read the old scale: they met above, or there is only this one)
+    if (wu == 0 && lane == 0) *scale_at = (bad || signbit(was)) ? -now : now;
+  }
+}
+
+template <typename T, int HD>
+int launch_fast(const Store& p, long long segments, cudaStream_t stream) {
+  const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
+  if (p.step.one_each) {
+    constexpr int SLOTS = 128 / (HD / 8);
+    gb_launch(kv8_store_rows_kernel<T, HD>, dim3((slots + SLOTS - 1) / SLOTS, p.step.n_requests), dim3(128), 0, stream, p);
+    return GB_OK;
+  }
+  // heads of a block: whole rounds of its warps, as many as leave four blocks for every SM
+  const int units = 8 / (p.page_size / 16), rounds = (slots + units - 1) / units;
+  long long shares = (4 * 148 + segments - 1) / segments;
+  if (shares > rounds) shares = rounds;
+  const int per_block = units * (int)((rounds + shares - 1) / shares);
+  const size_t smem = p.rotary ? (size_t)p.page_size * (HD / 2) * sizeof(float2) : 0;
+  static bool attr_set = false;
+  if (!attr_set) {
+    GB_CUDA(cudaFuncSetAttribute(kv8_store_pages_kernel<T, HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, 128 * (HD / 2) * 8));
+    attr_set = true;
+  }
+  gb_launch(kv8_store_pages_kernel<T, HD>, dim3((unsigned)segments, (slots + per_block - 1) / per_block), dim3(256), smem, stream, p, per_block);
+  return GB_OK;
+}
+
+// Whether the kernels above take a call: what they hold in registers, and sixteen bytes at a time.
+bool fast(const Store& p, int dtype) {
+  const int wpu = p.page_size / 16;
+  const uintptr_t size = dtype == GB_BF16 ? 2 : 4;
+  return (p.hd == 64 || p.hd == 128) && (p.rotary == nullptr || (p.rotary_dim == p.hd && !p.adjacent)) &&
+         (p.step.one_each || (p.page_size % 16 == 0 && (wpu == 1 || wpu == 2 || wpu == 4 || wpu == 8))) &&
+         (((uintptr_t)p.rows | (uintptr_t)p.part | (uintptr_t)p.q_out) & 15) == 0 && (p.ld * size) % 16 == 0;
+}
+
 }  // namespace
 
 GB_OP(gb_op_kv8_store) {
@@ -201,7 +494,12 @@ GB_OP(gb_op_kv8_store) {
   // upper bound of the pages written to: sum_r (pages of its tokens + 1 for beginning inside one)
   const long long segments = p.step.one_each ? p.step.n_requests
                                              : (long long)p.step.n_tokens / p.page_size + 2ll * p.step.n_requests;
-  int rc = dtype == GB_F32 ? launch_any<float>(p, segments, ctx->stream) : launch_any<bf16>(p, segments, ctx->stream);
+  int rc;
+  if (fast(p, dtype))
+    rc = p.hd == 64 ? (dtype == GB_F32 ? launch_fast<float, 64>(p, segments, ctx->stream) : launch_fast<bf16, 64>(p, segments, ctx->stream))
+                    : (dtype == GB_F32 ? launch_fast<float, 128>(p, segments, ctx->stream) : launch_fast<bf16, 128>(p, segments, ctx->stream));
+  else
+    rc = dtype == GB_F32 ? launch_any<float>(p, segments, ctx->stream) : launch_any<bf16>(p, segments, ctx->stream);
   if (rc != GB_OK) return rc;
   GB_CHECK_LAUNCH("kv8_store");
   return 1;
