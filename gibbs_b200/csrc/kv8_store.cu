@@ -156,90 +156,104 @@ int launch_any(const Store& p, long long segments, cudaStream_t stream) {
 }
 
 // ---------------------------------------------------------------- heads of 64 or 128, the rotation over the whole head (or none)
-// HD / 8 threads share a row, eight neighbouring values each: sixteen bytes of bfloat16 in, eight bytes of numbers out.  The sum of
-// squares and the rotation's partner (HD / 2 further) come from the neighbours by shuffles.
+// HD / 8 threads share a row, and a thread has the pairs that the rotation turns: entries 4 s .. 4 s + 3 and the four HD / 2 further,
+// so that nothing is exchanged but the sum of squares.
 template <typename T>
+__device__ __forceinline__ void load4(const T* src, float* v) {
+  if constexpr (sizeof(T) == 2) {
+    const uint2 w = *reinterpret_cast<const uint2*>(src);
+    v[0] = __uint_as_float(w.x << 16); v[1] = __uint_as_float(w.x & 0xffff0000u);
+    v[2] = __uint_as_float(w.y << 16); v[3] = __uint_as_float(w.y & 0xffff0000u);
+  } else {
+    const float4 a = *reinterpret_cast<const float4*>(src);
+    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w;
+  }
+}
+template <typename T>
+__device__ __forceinline__ void store4(T* dst, const float* v) {
+  if constexpr (sizeof(T) == 2) {
+    const __nv_bfloat162 a = __floats2bfloat162_rn(v[0], v[1]), b = __floats2bfloat162_rn(v[2], v[3]);
+    *reinterpret_cast<uint2*>(dst) = make_uint2(*reinterpret_cast<const uint32_t*>(&a), *reinterpret_cast<const uint32_t*>(&b));
+  } else {
+    *reinterpret_cast<float4*>(dst) = make_float4(v[0], v[1], v[2], v[3]);
+  }
+}
+// Columns col .. col + 3 and col + HD / 2 .. of a row.
+template <typename T, int HD>
 __device__ __forceinline__ void load8(const Store& p, int row, int col, float* v) {
   if (p.splits > 0) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) v[e] = 0.f;
     const float* src = p.part + (size_t)row * p.ld + col;
     for (int s = 0; s < p.splits; ++s, src += p.part_stride) {
-      const float4 a = ldcg_now(reinterpret_cast<const float4*>(src)), b = ldcg_now(reinterpret_cast<const float4*>(src) + 1);
+      const float4 a = ldcg_now(reinterpret_cast<const float4*>(src)), b = ldcg_now(reinterpret_cast<const float4*>(src + HD / 2));
       v[0] += a.x; v[1] += a.y; v[2] += a.z; v[3] += a.w;
       v[4] += b.x; v[5] += b.y; v[6] += b.z; v[7] += b.w;
     }
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      if (p.part_bias) v[e] += p.part_bias[col + e];
+      if (p.part_bias) v[e] += p.part_bias[col + e + (e < 4 ? 0 : HD / 2 - 4)];
       v[e] = to_f32(from_f32<T>(v[e]));                        // rounded where the product's own sum would have been
     }
     return;
   }
   const T* src = reinterpret_cast<const T*>(p.rows) + (size_t)row * p.ld + col;
-  if constexpr (sizeof(T) == 2) {
-    const uint4 raw = *reinterpret_cast<const uint4*>(src);
-    const uint32_t w[4] = {raw.x, raw.y, raw.z, raw.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v[2 * e] = __uint_as_float(w[e] << 16);
-      v[2 * e + 1] = __uint_as_float(w[e] & 0xffff0000u);
-    }
-  } else {
-    const float4 a = reinterpret_cast<const float4*>(src)[0], b = reinterpret_cast<const float4*>(src)[1];
-    v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-  }
+  load4<T>(src, v);
+  load4<T>(src + HD / 2, v + 4);
 }
-template <typename T>
-__device__ __forceinline__ void store8(T* dst, const float* v) {
-  if constexpr (sizeof(T) == 2) {
-    uint32_t w[4];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const __nv_bfloat162 b = __floats2bfloat162_rn(v[2 * e], v[2 * e + 1]);
-      w[e] = *reinterpret_cast<const uint32_t*>(&b);
-    }
-    *reinterpret_cast<uint4*>(dst) = make_uint4(w[0], w[1], w[2], w[3]);
-  } else {
-    reinterpret_cast<float4*>(dst)[0] = make_float4(v[0], v[1], v[2], v[3]);
-    reinterpret_cast<float4*>(dst)[1] = make_float4(v[4], v[5], v[6], v[7]);
-  }
-}
-// Norm (gain: this thread's eight, or none) and rotation (cs: the row's HD / 2 pairs of cos and sin, or null) of a row whose eight
-// values v this thread has; `sub` is the thread's place in the row.  All lanes of the warp take part.
+// Norm (gain: this thread's eight) and rotation (cs: cos and sin of this thread's four pairs, or null) of a row whose eight values
+// v this thread has.  All lanes of the warp take part.
 template <int HD>
-__device__ __forceinline__ void norm_rotate(float* v, const float* gain, bool norm, float eps, const float2* cs, int sub) {
+__device__ __forceinline__ void norm_rotate(float* v, const float* gain, bool norm, float eps, const float2* cs) {
   constexpr int TPR = HD / 8;
-  float ss = 0.f;
+  if (norm) {                                                  // (the same for the threads of a row)
+    float ss = 0.f;
 #pragma unroll
-  for (int e = 0; e < 8; ++e) ss += v[e] * v[e];
+    for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
+    const unsigned row = TPR == 8 ? 0xffu << (threadIdx.x & 24) : 0xffffu << (threadIdx.x & 16);
 #pragma unroll
-  for (int o = TPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-  if (norm) {
-    const float scale = 1.0f / sqrtf(ss * (1.f / HD) + eps);
+    for (int o = TPR / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(row, ss, o);
+    const float scale = rsqrtf(ss * (1.f / HD) + eps);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = v[e] * scale * gain[e];
+    for (int e = 0; e < 8; ++e) v[e] *= scale * gain[e];
   }
-  float w[8];
-#pragma unroll
-  for (int e = 0; e < 8; ++e) w[e] = __shfl_xor_sync(0xffffffffu, v[e], TPR / 2);
   if (cs != nullptr) {
-    const bool lower = sub < TPR / 2;
-    const float4* c4 = reinterpret_cast<const float4*>(cs + (lower ? sub : sub - TPR / 2) * 8);
+    const float4 a = reinterpret_cast<const float4*>(cs)[0], b = reinterpret_cast<const float4*>(cs)[1];
+    const float c[4] = {a.x, a.z, b.x, b.z}, s[4] = {a.y, a.w, b.y, b.w};
 #pragma unroll
-    for (int e = 0; e < 8; e += 2) {
-      const float4 t = c4[e / 2];                              // cos, sin of two pairs
-      v[e] = lower ? v[e] * t.x - w[e] * t.y : w[e] * t.y + v[e] * t.x;
-      v[e + 1] = lower ? v[e + 1] * t.z - w[e + 1] * t.w : w[e + 1] * t.w + v[e + 1] * t.z;
+    for (int e = 0; e < 4; ++e) {
+      const float lo = v[e], hi = v[e + 4];
+      v[e] = lo * c[e] - hi * s[e];
+      v[e + 4] = lo * s[e] + hi * c[e];
     }
   }
 }
+// The largest magnitude among a thread's eight (and `amax`).  A sum of squares says in one comparison that all is finite and far
+// below what a page holds; only where it does not, the values are looked at one by one.
 __device__ __forceinline__ void magnitude8(const float* v, float& amax, bool& bad) {
+  float ss = 0.f, top = amax;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    ss = fmaf(v[e], v[e], ss);
+    top = fmaxf(top, fabsf(v[e]));
+  }
+  if (ss <= 1e30f) {
+    amax = top;
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
     if (holdable(v[e])) amax = fmaxf(amax, fabsf(v[e]));
     else bad = true;
   }
+}
+// Four numbers; `bad`: some value of the page is not one that it holds.
+__device__ __forceinline__ uint32_t pack4(const float* v, float inv, bool bad) {
+  if (bad) return (uint32_t)pack2(v[0], v[1], inv) | (uint32_t)pack2(v[2], v[3], inv) << 16;
+  unsigned short a, b;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(a) : "f"(v[1] * inv), "f"(v[0] * inv));
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(b) : "f"(v[3] * inv), "f"(v[2] * inv));
+  return (uint32_t)a | (uint32_t)b << 16;
 }
 
 // Steps in which every request brings one token: a row is a unit, and 256 / HD of a block's 128 threads' rows make a warp's.  What
@@ -269,7 +283,7 @@ __global__ void __launch_bounds__(128) kv8_store_rows_kernel(const Store p) {
   float gain[8];
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    gain[e] = norm ? gain_at[sub * 8 + e] : 1.f;
+    gain[e] = norm ? gain_at[sub * 4 + e + (e < 4 ? 0 : HD / 2 - 4)] : 1.f;
     gb_pin(gain[e]);
   }
   gb_pin(page);
@@ -279,10 +293,10 @@ __global__ void __launch_bounds__(128) kv8_store_rows_kernel(const Store p) {
   const int kvh = active && !is_q ? (slot - p.heads) % p.kv_heads : 0;
   const bool there = page >= 0 && page < p.n_pages;
   float* scale_at = (is_k ? p.k_scales : p.v_scales) + (there ? (size_t)page * p.kv_heads + kvh : 0);
-  if (active) load8<T>(p, row, slot * HD + sub * 8, v);
+  if (active) load8<T, HD>(p, row, slot * HD + sub * 4, v);
   if (there && held > 0) was = *scale_at;
   __syncthreads();                                             // the angles
-  norm_rotate<HD>(v, gain, norm, p.eps, active && (is_q || is_k) && p.rotary ? cs : nullptr, sub);
+  norm_rotate<HD>(v, gain, norm, p.eps, active && (is_q || is_k) && p.rotary ? cs + sub * 4 : nullptr);
   float amax = 0.f;
   bool bad = false;
   magnitude8(v, amax, bad);
@@ -293,24 +307,28 @@ __global__ void __launch_bounds__(128) kv8_store_rows_kernel(const Store p) {
   }
   if (!active) return;
   if (is_q) {
-    store8<T>(reinterpret_cast<T*>(p.q_out) + ((size_t)row * p.heads + slot) * HD + sub * 8, v);
+    T* q = reinterpret_cast<T*>(p.q_out) + ((size_t)row * p.heads + slot) * HD + sub * 4;
+    store4<T>(q, v);
+    store4<T>(q + HD / 2, v + 4);
     return;
   }
   if (!there) {
     if (sub == 0) atomicExch(p.status, STATUS_BAD_PAGE_WRITE);
     return;
   }
-  uint8_t* dst = (is_k ? p.k_pages : p.v_pages) + ((size_t)page * p.kv_heads + kvh) * p.page_size * HD + sub * 8;
+  uint8_t* dst = (is_k ? p.k_pages : p.v_pages) + ((size_t)page * p.kv_heads + kvh) * p.page_size * HD;
   const float now = fmaxf(fabsf(was), scale_for(amax)), inv = inverse(now);
   if (held > 0 && fabsf(was) < now) {
     const float ratio = fabsf(was) * inv;
 #pragma unroll 4
     for (int i = 0; i < held; ++i) {
-      uint2* at = reinterpret_cast<uint2*>(dst + (size_t)i * HD);
+      uint2* at = reinterpret_cast<uint2*>(dst + (size_t)i * HD + sub * 8);
       *at = again8(*at, ratio);
     }
   }
-  *reinterpret_cast<uint2*>(dst + (size_t)held * HD) = pack8(v, inv);
+  uint32_t* at = reinterpret_cast<uint32_t*>(dst + (size_t)held * HD + sub * 4);
+  at[0] = pack4(v, inv, bad);
+  at[HD / 8] = pack4(v + 4, inv, bad);
   if (sub == 0) *scale_at = (bad || signbit(was)) ? -now : now;
 }
 
@@ -318,7 +336,7 @@ __global__ void __launch_bounds__(128) kv8_store_rows_kernel(const Store p) {
 // head) is held in registers by page_size / 16 warps, sixteen rows each, from the load to the store, so a row is read once; its
 // angles are worked out once a block into shared memory.
 template <typename T, int HD>
-__global__ void __launch_bounds__(256) kv8_store_pages_kernel(const Store p, int per_block) {
+__global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) kv8_store_pages_kernel(const Store p, int per_block) {
   constexpr int TPR = HD / 8, RPP = 32 / TPR, PASSES = 16 / RPP;       // threads of a row, rows of a pass, passes of sixteen rows
   extern __shared__ __align__(16) float2 cs_all[];                     // [new rows][HD / 2]
   __shared__ float top_of[8];
@@ -363,11 +381,11 @@ __global__ void __launch_bounds__(256) kv8_store_pages_kernel(const Store p, int
       mine[i] = active && o >= from && o < to;
 #pragma unroll
       for (int e = 0; e < 8; ++e) v[i][e] = 0.f;
-      if (mine[i]) load8<T>(p, row0 + o, slot * HD + sub * 8, v[i]);
+      if (mine[i]) load8<T, HD>(p, row0 + o, slot * HD + sub * 4, v[i]);
     }
     float gain[8];
 #pragma unroll
-    for (int e = 0; e < 8; ++e) gain[e] = gain_at ? gain_at[sub * 8 + e] : 1.f;
+    for (int e = 0; e < 8; ++e) gain[e] = gain_at ? gain_at[sub * 4 + e + (e < 4 ? 0 : HD / 2 - 4)] : 1.f;
     float was = 0.f;
     float* scale_at = (is_k ? p.k_scales : p.v_scales) + (there && !is_q ? (size_t)page * p.kv_heads + kvh : 0);
     if (active && !is_q && from > 0) was = *scale_at;
@@ -377,9 +395,13 @@ __global__ void __launch_bounds__(256) kv8_store_pages_kernel(const Store p, int
     for (int i = 0; i < PASSES; ++i) {
       const int o = 16 * wu + i * RPP + lane / TPR;
       norm_rotate<HD>(v[i], gain, gain_at != nullptr, p.eps,
-                      (is_q || is_k) && p.rotary ? cs_all + (size_t)(mine[i] ? o - from : 0) * (HD / 2) : nullptr, sub);
+                      (is_q || is_k) && p.rotary ? cs_all + (mine[i] ? o - from : 0) * (HD / 2) + sub * 4 : nullptr);
       if (is_q) {
-        if (mine[i]) store8<T>(reinterpret_cast<T*>(p.q_out) + ((size_t)(row0 + o) * p.heads + slot) * HD + sub * 8, v[i]);
+        if (mine[i]) {
+          T* q = reinterpret_cast<T*>(p.q_out) + ((size_t)(row0 + o) * p.heads + slot) * HD + sub * 4;
+          store4<T>(q, v[i]);
+          store4<T>(q + HD / 2, v[i] + 4);
+        }
       } else if (mine[i]) {
         magnitude8(v[i], amax, bad);
       }
@@ -400,16 +422,21 @@ __global__ void __launch_bounds__(256) kv8_store_pages_kernel(const Store p, int
       __syncthreads();
     }
     if (!active || is_q) continue;
-    uint8_t* dst = (is_k ? p.k_pages : p.v_pages) + ((size_t)page * p.kv_heads + kvh) * p.page_size * HD + sub * 8;
+    uint8_t* dst = (is_k ? p.k_pages : p.v_pages) + ((size_t)page * p.kv_heads + kvh) * p.page_size * HD;
     const float now = fmaxf(fabsf(was), scale_for(amax)), inv = inverse(now);
     const bool grown = from > 0 && fabsf(was) < now;
     const float ratio = fabsf(was) * inv;
 #pragma unroll
     for (int i = 0; i < PASSES; ++i) {
       const int o = 16 * wu + i * RPP + lane / TPR;
-      uint2* at = reinterpret_cast<uint2*>(dst + (size_t)o * HD);
-      if (mine[i]) *at = pack8(v[i], inv);
-      else if (grown && o < from) *at = again8(*at, ratio);
+      if (mine[i]) {
+        uint32_t* at = reinterpret_cast<uint32_t*>(dst + o * HD + sub * 4);
+        at[0] = pack4(v[i], inv, bad);
+        at[HD / 8] = pack4(v[i] + 4, inv, bad);
+      } else if (grown && o < from) {
+        uint2* at = reinterpret_cast<uint2*>(dst + o * HD + sub * 8);
+        *at = again8(*at, ratio);
+      }
     }
     // (every warp of the unit has read the old scale: they met above, or there is only this one)
     if (wu == 0 && lane == 0) *scale_at = (bad || signbit(was)) ? -now : now;
