@@ -20,7 +20,7 @@ from typing import Optional
 
 import torch
 
-from . import _f32vec, _launched, _need_cuda, _rotary_table, _rows, device_status, dtype_code, raw_stream
+from . import BF16, F32, _STATUS, _f32vec, _launched, _need_cuda, _rotary_table, _rows, device_status, dtype_code, raw_stream
 from .library import KernelError, check, library
 
 LIBRARY = "kv8"
@@ -73,7 +73,7 @@ class Pages:
         if k.data_ptr() % 16 or v.data_ptr() % 16:
             raise KernelError("8-bit pages: keys and values begin at 16-byte boundaries")
         self.k, self.v, self.k_scales, self.v_scales = k, v, k_scales, v_scales
-        self.device = k.device
+        self.device, self.index = k.device, k.get_device()
         self.addresses = (k.data_ptr(), v.data_ptr(), k_scales.data_ptr(), v_scales.data_ptr())
 
     def tensors(self) -> tuple:
@@ -89,36 +89,58 @@ def check_head_dim(head_dim: int) -> None:
         raise KernelError(f"an 8-bit cache holds heads of a multiple of 8 entries up to {MAX_HEAD_DIM}, not {head_dim}")
 
 
-def _call(operation: int, device: torch.device, a, f0: float, step, part=None) -> None:
-    run = _FN.get("run")
-    if run is None:
-        run = _FN["run"] = library(LIBRARY).gb_kv8_run
-        run.argtypes, run.restype = [ctypes.c_char_p], ctypes.c_int
+def _run():
+    run = _FN["run"] = library(LIBRARY).gb_kv8_run
+    run.argtypes, run.restype = [ctypes.c_char_p], ctypes.c_int
+    return run
+
+
+def _call(operation: int, index: int, device: torch.device, a, f0: float, step, part=None) -> None:
     n, r, longest = step.n_tokens, step.n_requests, step.max_q_len
     ws, splits, bias = 0, 0, 0
     if part is not None:
         ws, splits, bias = part.ws.data_ptr(), part.ws.shape[0], 0 if part.bias is None else part.bias.data_ptr()
-    rc = run(_WORDS.pack(operation, raw_stream(device), device_status(device).data_ptr(), n, r, 0, longest, step.max_ctx_len,
-                         1 if longest == 1 and n == r else 0, 0, 0, 0, step.q_start.data_ptr(), step.q_len.data_ptr(),
-                         step.start_pos.data_ptr(), ws, splits, bias, f0, *a))
+    status = _STATUS.get(index)
+    rc = (_FN.get("run") or _run())(
+        _WORDS.pack(operation, raw_stream(device), (device_status(device) if status is None else status).data_ptr(), n, r, 0, longest,
+                    step.max_ctx_len, 1 if longest == 1 and n == r else 0, 0, 0, 0, step.q_start.data_ptr(), step.q_len.data_ptr(),
+                    step.start_pos.data_ptr(), ws, splits, bias, f0, *a))
     if rc < 0:
         check(library(LIBRARY), rc)
     _launched(rc)
 
 
-_I32 = torch.int32
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 
 
-def _check_step(step, block_table: torch.Tensor, rows: int, device: torch.device, what: str) -> None:
+def _is(ok: bool, message: str) -> None:
+    if not ok:
+        raise KernelError(message)
+
+
+# The checks of a call are made twice over: as one expression, which is what a good call costs (a decode step makes a dozen of
+# them), and one by one with their messages where that expression is false.
+
+def _step_ok(step, block_table, rows: int, index: int) -> bool:
+    n, a, b, c = step.n_requests, step.q_start, step.q_len, step.start_pos
+    return (a.dtype is _I32 and b.dtype is _I32 and c.dtype is _I32 and a.get_device() == index and b.get_device() == index
+            and c.get_device() == index and a.is_contiguous() and b.is_contiguous() and c.is_contiguous() and a.numel() >= n
+            and b.numel() >= n and c.numel() >= n and block_table.dtype is _I32 and block_table.get_device() == index
+            and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[0] >= n and rows >= step.n_tokens)
+
+
+def _refuse_step(step, block_table, rows: int, index: int, what: str) -> None:
     n = step.n_requests
     for t in (step.q_start, step.q_len, step.start_pos):
-        if t.dtype is not _I32 or t.device != device or not t.is_contiguous() or t.numel() < n:
-            raise KernelError(f"{what}: q_start, q_len and start_pos are {n} contiguous int32 values on {device}")
-    if block_table.dtype is not _I32 or block_table.device != device or block_table.dim() != 2 \
-            or not block_table.is_contiguous() or block_table.shape[0] < n:
-        raise KernelError(f"{what}: the block table is contiguous int32 [{n} requests, entries] on {device}")
-    if rows < step.n_tokens:
-        raise KernelError(f"{what}: {rows} rows, the step has {step.n_tokens} tokens")
+        _is(t.dtype is _I32 and t.get_device() == index and t.is_contiguous() and t.numel() >= n,
+            f"{what}: q_start, q_len and start_pos are {n} contiguous int32 values on cuda:{index}")
+    _is(block_table.dtype is _I32 and block_table.get_device() == index and block_table.dim() == 2 and block_table.is_contiguous()
+        and block_table.shape[0] >= n, f"{what}: the block table is contiguous int32 [{n} requests, entries] on cuda:{index}")
+    _is(rows >= step.n_tokens, f"{what}: {rows} rows, the step has {step.n_tokens} tokens")
+
+
+def _vector_ok(t, n: int, index: int) -> bool:
+    return t is None or (t.dtype is _F32 and t.is_contiguous() and t.numel() == n and t.get_device() == index)
 
 
 def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head_dim: int, q_gain: Optional[torch.Tensor],
@@ -126,68 +148,92 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
                        adjacent_pairs: bool, step, block_table: torch.Tensor, pages: Optional[Pages]) -> torch.Tensor:
     """As ``ops.qk_norm_rope_store`` over an 8-bit cache: per-head RMSNorm (with gains) and rotation of q and k; q goes to
     ``q_out`` [tokens, heads * head_dim], k and v into their pages.  ``qkv``: rows [q heads | k heads | v heads], or the
-    ``ops.Partials`` of their product.  ``pages`` None: rows of q alone (a layer that reads another layer's cache).  Only
-    rows of the step's tokens are read or written."""
-    part = qkv if not isinstance(qkv, torch.Tensor) else None
+    ``ops.Partials`` of their product.  ``inv_freq``: rotary_dim / 2 frequencies, or those and the factor on cosines and sines
+    behind them.  ``pages`` None: rows of q alone (a layer that reads another layer's cache).  Only rows of the step's tokens
+    are read or written."""
+    part = None if isinstance(qkv, torch.Tensor) else qkv
     x = qkv if part is None else part.ws
-    _need_cuda(x, q_out, q_gain, k_gain, inv_freq)
-    if heads <= 0 or kv_heads <= 0:
-        raise KernelError(f"kv8 store: {heads} heads, {kv_heads} kv heads")
-    check_head_dim(head_dim)
-    cols = (heads + (2 * kv_heads if pages is not None else 0)) * head_dim
-    if part is not None:
-        if x.dtype != torch.float32 or not x.is_contiguous() or x.dim() != 3 or x.shape[1:] != (step.n_tokens, cols) \
-                or part.dtype != torch.bfloat16:
-            raise KernelError(f"kv8 store: partial tiles [splits, {step.n_tokens}, {cols}] float32 of a bfloat16 product expected")
-        _f32vec(part.bias, cols, "qkv bias")
-        rows, ld, dtype = x.shape[1], cols, torch.bfloat16
+    index, cols = x.get_device(), (heads + (2 * kv_heads if pages is not None else 0)) * head_dim
+    if inv_freq is not None and inv_freq.numel() != rotary_dim // 2 + 1 and not rotary_dim % 2:
+        inv_freq = _rotary_table(inv_freq, rotary_dim)
+    if part is None:
+        shape, stride = x.shape, x.stride()
+        good = len(shape) == 2 and (stride[1] == 1 or shape[1] == 1) and shape[1] >= cols and (x.dtype is _BF16 or x.dtype is _F32)
+        rows, ld, dtype = shape[0], stride[0], x.dtype
     else:
-        rows, ld, dtype = x.shape[0], _rows(x, "qkv"), x.dtype
-        if x.shape[1] < cols:
-            raise KernelError(f"kv8 store: rows of {x.shape[1]} columns, {cols} needed")
-    code = dtype_code(dtype)
-    if q_out.dtype != dtype or q_out.dim() != 2 or q_out.shape[1] != heads * head_dim or q_out.shape[0] < step.n_tokens \
-            or not q_out.is_contiguous():
-        raise KernelError(f"kv8 store: q_out is contiguous {dtype} [tokens, {heads * head_dim}]")
-    _f32vec(q_gain, head_dim, "q gain"), _f32vec(k_gain, head_dim, "k gain")
-    if inv_freq is not None and (rotary_dim % 2 or not 0 <= rotary_dim <= head_dim):
-        raise KernelError(f"kv8 store: a rotation over {rotary_dim} of {head_dim} entries")
-    table = _rotary_table(inv_freq, rotary_dim)
-    _check_step(step, block_table, rows, x.device, "kv8 store")
+        rows, ld, dtype = step.n_tokens, cols, _BF16
+        good = (x.dtype is _F32 and x.is_contiguous() and x.dim() == 3 and tuple(x.shape[1:]) == (rows, cols)
+                and part.dtype is _BF16 and _vector_ok(part.bias, cols, index))
+    if not (good and index >= 0 and heads > 0 and kv_heads > 0 and not head_dim % 8 and 8 <= head_dim <= MAX_HEAD_DIM
+            and q_out.dtype is dtype and q_out.get_device() == index and q_out.dim() == 2 and q_out.shape[1] == heads * head_dim
+            and q_out.shape[0] >= step.n_tokens and q_out.is_contiguous() and _vector_ok(q_gain, head_dim, index)
+            and _vector_ok(k_gain, head_dim, index) and (inv_freq is None or (
+                not rotary_dim % 2 and 0 <= rotary_dim <= head_dim and _vector_ok(inv_freq, rotary_dim // 2 + 1, index)))
+            and (pages is None or (pages.kv_heads == kv_heads and pages.head_dim == head_dim and pages.index == index))
+            and _step_ok(step, block_table, rows, index)):
+        _refuse_store(x, part, good, rows, cols, q_out, heads, kv_heads, head_dim, q_gain, k_gain, inv_freq, rotary_dim, step,
+                      block_table, pages, index, dtype)
     if pages is not None:
-        if (pages.kv_heads, pages.head_dim) != (kv_heads, head_dim) or pages.device != x.device:
-            raise KernelError(f"kv8 store: the pages hold {pages.kv_heads} kv heads of {pages.head_dim} on {pages.device}")
         k, v, ks, vs = pages.addresses
         n_pages, page_size = pages.n_pages, pages.page_size
     else:
         k = v = ks = vs = n_pages = 0
         page_size = 16
-    a = (x.data_ptr() if part is None else 0, ld, code, q_out.data_ptr(), 0 if q_gain is None else q_gain.data_ptr(),
-         0 if k_gain is None else k_gain.data_ptr(), 0 if table is None else table.data_ptr(), rotary_dim if table is not None else 0,
-         1 if adjacent_pairs else 0, k, v, ks, vs, n_pages, page_size, heads, kv_heads, head_dim, block_table.data_ptr(),
-         block_table.shape[1])
-    _call(0, x.device, a, eps, step, part)
+    _call(0, index, x.device, (
+        x.data_ptr() if part is None else 0, ld, BF16 if dtype is _BF16 else F32, q_out.data_ptr(),
+        0 if q_gain is None else q_gain.data_ptr(), 0 if k_gain is None else k_gain.data_ptr(),
+        0 if inv_freq is None else inv_freq.data_ptr(), 0 if inv_freq is None else rotary_dim, 1 if adjacent_pairs else 0, k, v, ks,
+        vs, n_pages, page_size, heads, kv_heads, head_dim, block_table.data_ptr(), block_table.shape[1]), eps, step, part)
     return q_out
+
+
+def _refuse_store(x, part, good, rows, cols, q_out, heads, kv_heads, head_dim, q_gain, k_gain, inv_freq, rotary_dim, step, block_table,
+                  pages, index, dtype) -> None:
+    _need_cuda(x, q_out, q_gain, k_gain, inv_freq, block_table)
+    _is(heads > 0 and kv_heads > 0, f"kv8 store: {heads} heads, {kv_heads} kv heads")
+    check_head_dim(head_dim)
+    if part is None:
+        dtype_code(x.dtype)
+        _is(good, f"kv8 store: rows of {cols} contiguous columns expected, got {tuple(x.shape)} strides {x.stride()}")
+    _is(good, f"kv8 store: partial tiles [splits, {rows}, {cols}] float32 of a bfloat16 product expected")
+    _is(q_out.dtype is dtype and q_out.dim() == 2 and q_out.shape[1] == heads * head_dim and q_out.shape[0] >= step.n_tokens
+        and q_out.is_contiguous(), f"kv8 store: q_out is contiguous {dtype} [tokens, {heads * head_dim}]")
+    _f32vec(q_gain, head_dim, "q gain"), _f32vec(k_gain, head_dim, "k gain")
+    _is(inv_freq is None or (not rotary_dim % 2 and 0 <= rotary_dim <= head_dim), f"kv8 store: a rotation over {rotary_dim} of {head_dim} entries")
+    _f32vec(inv_freq, rotary_dim // 2 + 1, "rotary table")
+    _is(pages is None or (pages.kv_heads, pages.head_dim, pages.index) == (kv_heads, head_dim, index),
+        "kv8 store: the pages hold another number of kv heads, other heads, or lie on another device")
+    _refuse_step(step, block_table, rows, index, "kv8 store")
+    raise KernelError(f"kv8 store: all tensors lie on cuda:{index}")
 
 
 def paged_attention(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, pages: Pages, block_table: torch.Tensor,
                     scale: float, window: int, out: torch.Tensor, step) -> torch.Tensor:
     """out[t, h, :] = softmax over visible keys of (q.K)*scale, times V, over an 8-bit cache; q may be a column slice of a
     wider row.  Rows of ``out`` behind the step's tokens are left as they are."""
-    _need_cuda(q, out)
-    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
-        raise KernelError(f"kv8 attention: {heads} heads are not a multiple of {kv_heads} kv heads")
-    cols, device = heads * head_dim, q.device
-    if q.dim() != 2 or out.dim() != 2 or q.shape[1] != cols or out.shape[1] != cols or q.dtype != out.dtype \
-            or out.shape[0] < step.n_tokens:
-        raise KernelError(f"kv8 attention: q and out are [tokens, {cols}] of one dtype")
-    if pages.kv_heads != kv_heads or pages.head_dim != head_dim or pages.device != device or out.device != device:
-        raise KernelError(f"kv8 attention: the pages hold {pages.kv_heads} kv heads of {pages.head_dim} on {pages.device}")
-    if window is None or window < 0:
-        raise KernelError(f"kv8 attention: a window of {window} keys (0: none)")
-    _check_step(step, block_table, q.shape[0], device, "kv8 attention")
+    index, cols, qs, os_, dtype = q.get_device(), heads * head_dim, q.stride(), out.stride(), q.dtype
+    if not (index >= 0 and heads > 0 and kv_heads > 0 and not heads % kv_heads and len(qs) == 2 and len(os_) == 2
+            and q.shape[1] == cols and out.shape[1] == cols and (qs[1] == 1 or cols == 1) and (os_[1] == 1 or cols == 1)
+            and out.dtype is dtype and (dtype is _BF16 or dtype is _F32) and out.shape[0] >= step.n_tokens and out.get_device() == index
+            and pages.kv_heads == kv_heads and pages.head_dim == head_dim and pages.index == index and window is not None and window >= 0
+            and _step_ok(step, block_table, q.shape[0], index)):
+        _refuse_attention(q, heads, kv_heads, head_dim, pages, block_table, window, out, step, index)
     k, v, ks, vs = pages.addresses
-    _call(1, device, (q.data_ptr(), _rows(q, "q"), dtype_code(q.dtype), out.data_ptr(), _rows(out, "out"), k, v, ks, vs,
-                      pages.n_pages, pages.page_size, heads, kv_heads, head_dim, block_table.data_ptr(), block_table.shape[1],
-                      window, 0, 0, 0), scale, step)
+    _call(1, index, q.device, (q.data_ptr(), qs[0], BF16 if dtype is _BF16 else F32, out.data_ptr(), os_[0], k, v, ks, vs, pages.n_pages,
+                               pages.page_size, heads, kv_heads, head_dim, block_table.data_ptr(), block_table.shape[1], window, 0, 0, 0),
+          scale, step)
     return out
+
+
+def _refuse_attention(q, heads, kv_heads, head_dim, pages, block_table, window, out, step, index) -> None:
+    _need_cuda(q, out, block_table)
+    _is(heads > 0 and kv_heads > 0 and not heads % kv_heads, f"kv8 attention: {heads} heads are not a multiple of {kv_heads} kv heads")
+    dtype_code(q.dtype)
+    _is(q.dim() == 2 and out.dim() == 2 and q.shape[1] == out.shape[1] == heads * head_dim and q.dtype is out.dtype
+        and out.shape[0] >= step.n_tokens, f"kv8 attention: q and out are [tokens, {heads * head_dim}] of one dtype")
+    _rows(q, "kv8 attention q"), _rows(out, "kv8 attention out")
+    _is((pages.kv_heads, pages.head_dim, pages.index) == (kv_heads, head_dim, index) and out.get_device() == index,
+        f"kv8 attention: the pages hold {pages.kv_heads} kv heads of {pages.head_dim} on {pages.device}")
+    _is(window is not None and window >= 0, f"kv8 attention: a window of {window} keys (0: none)")
+    _refuse_step(step, block_table, q.shape[0], index, "kv8 attention")
+    raise KernelError("kv8 attention: a call of these tensors is not taken")
