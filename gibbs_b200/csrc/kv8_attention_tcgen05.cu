@@ -662,10 +662,14 @@ int launch(const Attn& p, long long tiles, long long keys, cudaStream_t stream) 
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_tcgen05_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM));
     attr_set = true;
   }
-  // CTAs that share a tile's keys: as many as the SMs hold at a time, each with four key tiles at least
-  int parts = 1;
-  while (parts < 8 && tiles * p.kv_heads * parts * 2 <= 148 && (keys + KEYS - 1) / KEYS >= 8ll * parts) parts *= 2;
-  return launch_parts(kv8_attention_tcgen05_kernel<HD>, p, parts, tiles, THREADS, Cfg<HD>::SMEM, stream);
+  // CTAs that share a tile's keys: as many as the SMs hold at a time, each with four key tiles at least.  `tiles` is an upper bound
+  // that counts one for every request; the CTAs that have long walks are those of the longest portion, or of all tokens together.
+  const int two = 2 * (ROWS / (p.heads / p.kv_heads));
+  const long long longest = (p.step.max_q + two - 1) / two, all = p.step.n_tokens / two, walks = (longest > all ? longest : all) * p.kv_heads;
+  long long parts = 148 / walks, most = (keys + KEYS - 1) / KEYS / 4;
+  if (parts > most) parts = most;
+  parts = parts < 1 ? 1 : parts > 8 ? 8 : parts;
+  return launch_parts(kv8_attention_tcgen05_kernel<HD>, p, (int)parts, tiles, THREADS, Cfg<HD>::SMEM, stream);
 }
 
 }  // namespace

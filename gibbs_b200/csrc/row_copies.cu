@@ -6,7 +6,7 @@
 // one trip (eight 16-byte loads a lane in flight).  The pairs travel in the launch's arguments: no copy to the device goes in
 // front.  Bound by memory: every byte is read once and written once.
 #include <exception>
-#include <unordered_set>
+#include <vector>
 
 #include "common.cuh"
 
@@ -66,14 +66,19 @@ int check_pairs(int g, const int* pairs, int n, int rows) {
     return GB_OK;
   }
   try {
-    std::unordered_set<int> to;
-    to.reserve((size_t)n * 2);
-    for (int i = 0; i < n; ++i)
-      if (!to.insert(pairs[2 * i + 1]).second)
-        GB_FAIL(GB_ERR_ARG, "row copies: row %d of group %d is a destination twice", pairs[2 * i + 1], g);
-    for (int i = 0; i < n; ++i)
-      if (to.count(pairs[2 * i]))
-        GB_FAIL(GB_ERR_ARG, "row copies: row %d of group %d is a destination and a source", pairs[2 * i], g);
+    static thread_local std::vector<unsigned char> to;         // 1: a destination (all 0 between calls)
+    if (to.size() < (size_t)rows) to.resize((size_t)rows, 0);
+    int bad = -1, twice = 0;
+    for (int i = 0; i < n && bad < 0; ++i) {
+      if (to[pairs[2 * i + 1]]) bad = i, twice = 1;
+      to[pairs[2 * i + 1]] = 1;
+    }
+    for (int i = 0; i < n && bad < 0; ++i)
+      if (to[pairs[2 * i]]) bad = i;
+    for (int i = 0; i < n; ++i) to[pairs[2 * i + 1]] = 0;
+    if (bad >= 0)
+      GB_FAIL(GB_ERR_ARG, "row copies: row %d of group %d is a destination %s", pairs[2 * bad + (twice ? 1 : 0)], g,
+              twice ? "twice" : "and a source");
   } catch (const std::exception& e) {
     GB_FAIL(GB_ERR_ARG, "row copies: %s", e.what());
   }
