@@ -186,32 +186,43 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     constexpr int MINE = (GROUPS + CONVERTERS / 32 - 1) / (CONVERTERS / 32);
     const int w0 = warp - 8, piece = lane % PIECES, row_in = lane / PIECES;      // groups w0, w0 + 3, w0 + 6 < 8
     const int* bt = p.block_table + (size_t)r * p.bt_stride;
-    // lane i < 8: page of group i of a tile, -1 where nothing of it is visible (and in the other lanes)
+    // lane i < 8: page of group i of a tile, -1 where nothing of it is visible (and in the other lanes); as it comes from the table,
+    // and looked at only when it is needed, which is after its trip
     auto page_of = [&](int j) {
       const int key = (t_lo + j) * KEYS + lane * 16;
-      if (lane >= GROUPS || j >= n || key >= hi || key + 15 < lo) return -1;
-      const int page = bt[key >> p.page_shift];
-      if (page >= 0 && page < p.n_pages) return page;
+      return (lane >= GROUPS || j >= n || key >= hi || key + 15 < lo) ? -1 : bt[key >> p.page_shift] & 0x7fffffff;
+    };
+    auto checked = [&](int page) {
+      if (page < p.n_pages) return page;
       if (warp == 8) atomicExch(p.status, STATUS_BAD_PAGE_READ);
       return -1;
     };
     uint8_t* mine = sraw + lane * 16;
+    const uint32_t mine_at = smem_u32(mine) + w0 * 16 * HD;
     const size_t head = (size_t)kvh << p.page_shift;
-    // Asks for an item; what is not visible, or behind the context (which holds anything, and 0 * NaN is not 0), comes as zeros.
+    size_t at[MINE];                                          // where this warp's groups of the last tile asked for lie in the pool
+    int rows[MINE];                                            // how many rows from this lane's first on are there
+    // Asks for an item, K of a tile and then its V; what is not visible, or behind the context (which holds anything, and 0 * NaN is
+    // not 0), comes as zeros.
     auto request = [&](int it, int page) {
       if (it < 2 * n) {
+        if (!(it & 1)) {
+          const int key0 = (t_lo + (it >> 1)) * KEYS;
+#pragma unroll
+          for (int y = 0; y < MINE; ++y) {
+            const int g = w0 + y * (CONVERTERS / 32), pg = __shfl_sync(0xffffffffu, page, g), key = key0 + 16 * g;
+            at[y] = pg < 0 ? 0 : ((((size_t)pg * p.kv_heads) << p.page_shift) + head + (key & (p.page_size - 1))) * HD;
+            rows[y] = pg < 0 || g >= GROUPS ? 0 : hi - key - row_in;
+          }
+        }
         const uint8_t* pool = ((it & 1) ? p.v_pages : p.k_pages) + lane * 16;
-        const int key0 = (t_lo + (it >> 1)) * KEYS;
-        const uint32_t dst = smem_u32(mine) + (uint32_t)((it % C::STAGES) * C::RAW_TILE);
+        const uint32_t dst = mine_at + (uint32_t)((it % C::STAGES) * C::RAW_TILE);
 #pragma unroll
         for (int y = 0; y < MINE; ++y) {
-          const int g = w0 + y * (CONVERTERS / 32), pg = __shfl_sync(0xffffffffu, page, g), key = key0 + 16 * g;
-          if (g >= GROUPS) continue;
-          const uint8_t* src = pool + (pg < 0 ? 0 : ((((size_t)pg * p.kv_heads) << p.page_shift) + head + (key & (p.page_size - 1))) * HD);
-          const int rows = pg < 0 ? 0 : hi - key - row_in;     // (positive: there)
+          if (w0 + y * (CONVERTERS / 32) >= GROUPS) continue;
 #pragma unroll
           for (int i = 0; i < PER; ++i)
-            cp_async_16(dst + (uint32_t)(g * 16 * HD + i * 512), src + i * 512, rows > i * ROWS_STEP ? 16 : 0);
+            cp_async_16(dst + (uint32_t)(y * (CONVERTERS / 32) * 16 * HD + i * 512), pool + at[y] + i * 512, rows[y] > i * ROWS_STEP ? 16 : 0);
         }
       }
       asm volatile("cp.async.commit_group;" ::: "memory");
@@ -226,6 +237,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     };
     // pages of tile j, j + 1, ... (a request goes out at most STAGES items, two tiles, ahead)
     int pages[4] = {page_of(0), page_of(1), page_of(2), page_of(3)};
+#pragma unroll
+    for (int i = 0; i < 3; ++i) pages[i] = checked(pages[i]);
 #pragma unroll
     for (int it = 0; it < C::STAGES; ++it) request(it, pages[it >> 1]);
     scales(pages[0], ks, vs);
@@ -312,7 +325,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
       vs = vs_next;
       pages[0] = pages[1];
       pages[1] = pages[2];
-      pages[2] = pages[3];
+      pages[2] = checked(pages[3]);
       pages[3] = page_of(j + 4);
     }
     asm volatile("cp.async.wait_group 0;" ::: "memory");
