@@ -318,10 +318,13 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, t4 = lane & 3;
   const int part = (int)blockIdx.x % p.parts, unit = (int)blockIdx.x / p.parts, kvh = unit % p.kv_heads;
   Tile t;
-  if (!find_tile<RT>(p, unit / p.kv_heads, t)) return;         // (the same for every CTA of a cluster)
-  const int c_lo = t.lo / CK, chunks = (t.hi + CK - 1) / CK - c_lo;
+  const bool found = find_tile<RT>(p, unit / p.kv_heads, t);   // (the same for every CTA of a cluster)
+  const int c_lo = found ? t.lo / CK : 0, chunks = found ? (t.hi + CK - 1) / CK - c_lo : 0;
   const int parts = max(1, min(p.parts, (chunks + NW - 1) / NW));
-  if (part >= parts) return;                                   // (a thread that has left counts as arrived at the cluster's barriers)
+  if (!found || part >= parts) {                               // (a thread that has left counts as arrived at the cluster's barriers)
+    if (p.first) pdl_wait();
+    return;
+  }
   const int* bt = p.block_table + (size_t)t.r * p.bt_stride;
   const int stride = parts * NW, first = part * NW + warp;
   const int mine = first < chunks ? (chunks - 1 - first) / stride + 1 : 0;           // chunks of this warp
@@ -382,6 +385,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   gb_pin(row);
   gb_pin(page_ahead);
   pdl_wait();
+  if (p.first) pdl_trigger();
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i)
     if (i < mine) request(i);
@@ -735,13 +739,15 @@ GB_OP(gb_op_kv8_attention) {
   // Requests of more than FEW rows go to tcgen05, which takes 256 rows at a time; they have to lie on 16-byte boundaries.
   const bool wide = mma && (long long)p.step.max_q * group > FEW && group <= 64 && p.ldo % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
   p.few = 0x7fffffff;
-  int launched = 0;
-  if (wide) {
-    p.few = p.step.n_requests == 1 ? 0 : FEW;                  // (one request: all of it, whatever it brings)
+  p.first = p.second = 0;
+  if (wide && p.step.n_requests == 1) {
+    p.few = 0;                                                 // (all of it, whatever it brings)
     const int rc = kv8_attention_tcgen05(p, ctx->stream);
-    if (rc != GB_OK) return rc;
-    if (p.step.n_requests == 1) return 1;
-    launched = 1;
+    return rc == GB_OK ? 1 : rc;
+  }
+  if (wide) {
+    p.few = FEW;
+    p.first = 1;
   }
   // rows of a tile: with 8, a step of single tokens in groups of eight heads or fewer, and what stands beside wide portions (single
   // tokens as a rule); with 16, half as many passes over the keys
@@ -764,5 +770,9 @@ GB_OP(gb_op_kv8_attention) {
     rc = dtype == GB_F32 ? dispatch_any<float>(p, tiles, keys, ctx->stream) : dispatch_any<bf16>(p, tiles, keys, ctx->stream);
   if (rc != GB_OK) return rc;
   GB_CHECK_LAUNCH("kv8_attention");
-  return launched + 1;
+  if (!wide) return 1;
+  p.first = 0;
+  p.second = 1;
+  rc = kv8_attention_tcgen05(p, ctx->stream);
+  return rc == GB_OK ? 2 : rc;
 }

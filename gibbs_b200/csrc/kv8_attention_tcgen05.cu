@@ -126,7 +126,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     const int n = p.step.q_len[i];
     return n * group > p.few ? (n + 2 * tpt - 1) / (2 * tpt) : 0;
   }, tile);
-  if (r < 0) return;                                           // (the same for every CTA of a cluster)
+  if (r < 0) {                                                 // (the same for every CTA of a cluster)
+    if (p.second) pdl_wait();
+    return;
+  }
   const int qlen = p.step.q_len[r], start = p.step.start_pos[r], qstart = p.step.q_start[r];
   tile = (qlen + 2 * tpt - 1) / (2 * tpt) - 1 - tile;          // the tiles with the most keys first
   const int tok0 = tile * 2 * tpt, n_tok = min(2 * tpt, qlen - tok0);
@@ -135,7 +138,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   const int lo = (p.window > 0 && first - p.window + 1 > 0) ? first - p.window + 1 : 0;
   int t_lo = lo / KEYS, t_hi = (hi + KEYS - 1) / KEYS;
   const int parts = max(1, min(p.parts, (t_hi - t_lo) / 2));
-  if (part >= parts) return;                                   // (a thread that has left counts as arrived at the cluster's barriers)
+  if (part >= parts) {                                         // (a thread that has left counts as arrived at the cluster's barriers)
+    if (p.second) pdl_wait();
+    return;
+  }
   {
     const int whole = t_hi - t_lo, from = t_lo;
     t_lo = from + whole * part / parts;
@@ -173,7 +179,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   const uint32_t tmem = tmem_slot;
   const uint32_t tmem_s[2] = {tmem, tmem + KEYS}, tmem_o[2] = {tmem + 2 * KEYS, tmem + 2 * KEYS + HD};
   const uint32_t tmem_p[2] = {C::APART ? tmem + 2 * KEYS + 2 * HD : tmem, C::APART ? tmem + 2 * KEYS + 2 * HD + KEYS / 2 : tmem + KEYS};
-  pdl_wait();
+  if (!p.second) pdl_wait();
 
   if (warp >= 8 && warp < 11) {
     // ---- K and V: pages -> f16 tiles ----
@@ -666,6 +672,34 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   tc_fence_before();
   __syncthreads();
   if (warp == 11) tmem_dealloc(tmem_slot, 512);
+  if (p.second) pdl_wait();
+}
+
+constexpr int MAX_SHARES = 8;
+
+// How many clusters of `parts` CTAs the GPU holds at a time (a cluster lies within a part of the chip, so not all SMs can be had).
+template <int HD>
+int clusters_at_a_time(int parts) {
+  static int known[MAX_SHARES + 1] = {};                       // (a property of the kernel and the chip)
+  if (known[parts] == 0) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)(parts * 148));
+    cfg.blockDim = dim3(THREADS);
+    cfg.dynamicSmemBytes = Cfg<HD>::SMEM;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)parts;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    int n = 0;
+    if (cudaOccupancyMaxActiveClusters(&n, kv8_attention_tcgen05_kernel<HD>, &cfg) != cudaSuccess) {
+      cudaGetLastError();
+      n = 0;
+    }
+    known[parts] = n > 0 ? n : -1;
+  }
+  return known[parts];
 }
 
 template <int HD>
@@ -679,10 +713,11 @@ int launch(const Attn& p, long long tiles, long long keys, cudaStream_t stream) 
   // that counts one for every request; the CTAs that have long walks are those of the longest portion, or of all tokens together.
   const int two = 2 * (ROWS / (p.heads / p.kv_heads));
   const long long longest = (p.step.max_q + two - 1) / two, all = p.step.n_tokens / two, walks = (longest > all ? longest : all) * p.kv_heads;
-  long long parts = 148 / walks, most = (keys + KEYS - 1) / KEYS / 4;
-  if (parts > most) parts = most;
-  parts = parts < 1 ? 1 : parts > 8 ? 8 : parts;
-  return launch_parts(kv8_attention_tcgen05_kernel<HD>, p, (int)parts, tiles, THREADS, Cfg<HD>::SMEM, stream);
+  const long long most = (keys + KEYS - 1) / KEYS / 4;
+  int parts = 1;
+  for (int x = 2; x <= MAX_SHARES && x <= most; ++x)
+    if (walks <= clusters_at_a_time<HD>(x)) parts = x;
+  return launch_parts(kv8_attention_tcgen05_kernel<HD>, p, parts, tiles, THREADS, Cfg<HD>::SMEM, stream);
 }
 
 }  // namespace
