@@ -341,13 +341,12 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   constexpr int NONE = -1;
   auto page_of = [&](int n) {
     const int c = first + (n / NG) * stride, j = (c_lo + c) * CK + (n % NG) * 16;
-    if (c >= chunks || j >= t.hi || j + 15 < t.lo) return NONE;
-    const int page = bt[j >> p.page_shift];
-    if (page < 0 || page >= p.n_pages) {
-      atomicExch(p.status, STATUS_BAD_PAGE_READ);
-      return NONE;
-    }
-    return page;
+    return (c >= chunks || j >= t.hi || j + 15 < t.lo) ? NONE : bt[j >> p.page_shift] & 0x7fffffff;
+  };
+  auto checked = [&](int page) {                               // (apart from the lookup, so that its trip is not waited for there)
+    if (page < p.n_pages) return page;
+    atomicExch(p.status, STATUS_BAD_PAGE_READ);
+    return NONE;
   };
   auto row_of = [&](int n, int page) {
     const int j = (c_lo + first + (n / NG) * stride) * CK + (n % NG) * 16;
@@ -356,8 +355,9 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   // Requests run SLOTS chunks ahead of the products: `row` is of the 32 groups that are being requested, `ks`, `vs` of the 32 that
   // are being worked on, `ks_next`, `vs_next` of the former where they differ, `page_ahead` of the 32 behind those.
   int page = page_of(lane), page_ahead = page_of(32 + lane);
+  page = checked(page);
   int row = row_of(lane, page);
-  float ks_own = 0.f, vs_own = 0.f, ks_next = 0.f, vs_next = 0.f;
+  float ks_own = 0.f, vs_own = 0.f, ks_next = 0.f, vs_next = 0.f, lv_own = 0.f, inv_own = 0.f;
   auto scales_of = [&](int page_, float& ks, float& vs) {      // (0: no page)
     ks = vs = 0.f;
     if (page_ != NONE) {
@@ -367,8 +367,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   };
   uint8_t* ring = smem + warp * SLOTS * C::SLOT;
   // Requests the groups of the warp's chunk i.  A group without a page brings row 0 of the pool, which is never looked at.
-  auto request = [&](int i) {
-    const int slot = i % SLOTS;
+  auto request = [&](int i, int slot) {
     int at[NG];
 #pragma unroll
     for (int y = 0; y < NG; ++y) at[y] = max(0, __shfl_sync(0xffffffffu, row, (i * NG + y) & 31));
@@ -388,8 +387,10 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   if (p.first) pdl_trigger();
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i)
-    if (i < mine) request(i);
+    if (i < mine) request(i, i);
   scales_of(page, ks_own, vs_own);
+  lv_own = log2_of(vs_own);
+  inv_own = inverse(vs_own);
 
   // q: row g of each block, entries t4 * KB ... + KB, under its power of two.  In the lane's columns of S^T and O^T stand rows
   // 2t and 2t + 1 of each block.
@@ -449,10 +450,12 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int pos_first = t.pos(0), pos_last = t.pos(t.rows - 1);
   const int key_g = key_at(g), key_0 = key_at(2 * t4), key_1 = key_at(2 * t4 + 1);
   bool alive = true;
+  uint32_t marked = __ballot_sync(0xffffffffu, vs_own < 0.f);  // which of the 32 groups lie in pages with NaN among their values
 
+  int slot = 0, phase = 0;
   for (int i = 0; i < mine; ++i) {
-    const int n0 = i * NG, slot = i % SLOTS;
-    if (!__all_sync(0xffffffffu, sm100::mbar_wait(&full[warp][slot], (i / SLOTS) & 1))) {
+    const int n0 = i * NG;
+    if (!__all_sync(0xffffffffu, sm100::mbar_wait(&full[warp][slot], phase))) {
       alive = false;
       break;
     }
@@ -460,12 +463,11 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const uint8_t* vt = kt + NG * C::GROUP;
     const int j_chunk = (c_lo + first + i * stride) * CK;
     float s[NB][NG][4], inv[NG];
-    bool careful = false;                                      // some page of the chunk has NaN among its values
+    const bool careful = (marked >> (n0 & 31)) & ((1u << NG) - 1);     // some page of the chunk has NaN among its values
 #pragma unroll
     for (int y = 0; y < NG; ++y) {
-      const float ks = __shfl_sync(0xffffffffu, ks_own, (n0 + y) & 31), vs = __shfl_sync(0xffffffffu, vs_own, (n0 + y) & 31);
-      careful |= vs < 0.f;
-      inv[y] = inverse(vs);
+      const float ks = __shfl_sync(0xffffffffu, ks_own, (n0 + y) & 31), lv = __shfl_sync(0xffffffffu, lv_own, (n0 + y) & 31);
+      inv[y] = __shfl_sync(0xffffffffu, inv_own, (n0 + y) & 31);
       uint32_t w[2][KW];
 #pragma unroll
       for (int h = 0; h < 2; ++h) read_bytes<HD, C::KB>(kt + y * C::GROUP, key_g + 8 * h, t4 * C::KB, w[h]);
@@ -484,7 +486,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
       // x = score + log2(scale of V), -inf where a row does not see the key
       const int j0 = j_chunk + 16 * y;
       const bool full_ = ks != 0.f && j0 + 15 <= pos_first && (p.window <= 0 || j0 + p.window > pos_last);
-      const float lv = log2_of(vs), kf = fabsf(ks);
+      const float kf = fabsf(ks);
 #pragma unroll
       for (int b = 0; b < NB; ++b) {
         const float f0 = factor[b][0] * kf, f1 = factor[b][1] * kf;
@@ -610,15 +612,20 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     const int ahead = i + SLOTS;
     if (ahead < mine) {
       if (((ahead * NG) & 31) == 0) {
-        row = row_of(ahead * NG + lane, page_ahead);
-        scales_of(page_ahead, ks_next, vs_next);
+        const int next = checked(page_ahead);
+        row = row_of(ahead * NG + lane, next);
+        scales_of(next, ks_next, vs_next);
         page_ahead = page_of(ahead * NG + 32 + lane);
       }
-      request(ahead);
+      request(ahead, slot);
     }
+    if (++slot == SLOTS) slot = 0, phase ^= 1;
     if (((n0 + NG) & 31) == 0) {
       ks_own = ks_next;
       vs_own = vs_next;
+      lv_own = log2_of(vs_own);
+      inv_own = inverse(vs_own);
+      marked = __ballot_sync(0xffffffffu, vs_own < 0.f);
     }
   }
   pdl_trigger();       // (not earlier: CTAs of the next kernel beside these would leave its others unevenly spread over the SMs)
