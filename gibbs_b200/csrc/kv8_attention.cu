@@ -263,11 +263,11 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
 // the warp's own, and a copy costs an instruction instead of one for every lane and piece.  The rows are swizzled (128-byte
 // rows by the 16-byte piece XOR row, 64-byte rows by piece XOR row / 2) and the keys of a group take the places pi(0..15) of the
 // products: with these every fragment is read without a bank conflict.
-template <int HD> struct Mma {
-  static constexpr int NW = 4;
+template <int HD, int WARPS> struct Mma {
+  static constexpr int NW = WARPS;
   static constexpr int NG = 2;                                 // groups of a slot, taken together
   static constexpr int SLOTS = HD <= 64 ? 3 : 2;
-  static constexpr int CTAS = HD <= 64 ? 4 : 3;                // on an SM: by shared memory, and registers capped to that
+  static constexpr int CTAS = WARPS > 4 ? 1 : HD <= 64 ? 4 : 3;        // on an SM: by shared memory, and registers capped to that
   static constexpr int CK = 16 * NG;                           // keys of a chunk
   static constexpr int KB = HD / 4, VB = HD / 8;               // bytes of a lane's piece of a key, of a value
   static constexpr int GROUP = 16 * HD;                        // bytes of a group's keys
@@ -307,10 +307,10 @@ __device__ __forceinline__ uint32_t transposed(uint32_t v) {   // an 8 x 8 matri
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
-template <int HD, int NB>
-__global__ void __launch_bounds__(128, NB == 1 ? Mma<HD>::CTAS : 1)
+template <int HD, int NB, int WARPS>
+__global__ void __launch_bounds__(32 * WARPS, NB == 1 ? Mma<HD, WARPS>::CTAS : 1)
 kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, const Attn p) {
-  using C = Mma<HD>;
+  using C = Mma<HD, WARPS>;
   constexpr int RT = 8 * NB, NW = C::NW, NG = C::NG, CK = C::CK, KW = C::KB / 4, VW = C::VB / 4, SLOTS = C::SLOTS;
   extern __shared__ uint8_t smem_raw[];
   __shared__ uint64_t full[NW][SLOTS];
@@ -687,14 +687,18 @@ int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t st
   }
 }
 
-template <int HD, int NB>
-int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
-  using C = Mma<HD>;
+// Few tiles (a launch of few requests): one CTA of many warps for an SM, and a tile's keys shared by a cluster of them, as many as the
+// chip holds at a time.  (Clusters of four-warp CTAs come to lie three or four on an SM and leave others empty: 4 requests of 32,000
+// keys, 32 / 8 heads of 128, 55 us.)  Many tiles: CTAs of four warps, several on an SM, so that one's beginning and end lie beside the
+// others' work.
+template <int HD, int NB, int WARPS>
+int launch_mma_of(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
+  using C = Mma<HD, WARPS>;
   constexpr int SMEM = C::smem(8 * NB);
   static bool attr_set = false;
   if (!attr_set) {
-    GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
-    GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM));
+    GB_CUDA(cudaFuncSetAttribute(kv8_attention_mma_kernel<HD, NB, WARPS>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set = true;
   }
   CUtensorMap mk, mv;
@@ -702,8 +706,21 @@ int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stre
   constexpr CUtensorMapSwizzle SWIZZLE = HD == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
   if (!group_map(&mk, p.k_pages, rows, HD, SWIZZLE) || !group_map(&mv, p.v_pages, rows, HD, SWIZZLE))
     GB_FAIL(GB_ERR_CUDA, "kv8_attention: cuTensorMapEncodeTiled failed (%lld rows of %d)", rows, HD);
-  const int parts = key_parts(tiles * p.kv_heads, 148 * C::CTAS, (keys + C::CK - 1) / C::CK, C::NW);
-  return launch_parts(kv8_attention_mma_kernel<HD, NB>, p, parts, tiles, 32 * C::NW, SMEM, stream, mk, mv);
+  const long long chunks = (keys + C::CK - 1) / C::CK, ctas = tiles * p.kv_heads;
+  int parts = 1;
+  if (C::CTAS == 1) {
+    for (int x = 2; x <= MAX_PARTS && chunks > (long long)(x - 1) * C::NW; ++x)
+      if (ctas <= clusters_at_a_time(kv8_attention_mma_kernel<HD, NB, WARPS>, x, 32 * C::NW, SMEM)) parts = x;
+  } else {
+    parts = key_parts(ctas, 148 * C::CTAS, chunks, C::NW);
+  }
+  return launch_parts(kv8_attention_mma_kernel<HD, NB, WARPS>, p, parts, tiles, 32 * C::NW, SMEM, stream, mk, mv);
+}
+template <int HD, int NB>
+int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
+  // (tiles of 16 rows need twice the registers: eight warps)
+  constexpr int MANY = NB == 2 ? 8 : HD == 64 ? 16 : 12;
+  return tiles * p.kv_heads <= 148 ? launch_mma_of<HD, NB, MANY>(p, tiles, keys, stream) : launch_mma_of<HD, NB, 4>(p, tiles, keys, stream);
 }
 
 }  // namespace

@@ -63,6 +63,34 @@ static bool group_map(CUtensorMap* map, const void* pages, long long rows, int h
             swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+// How many clusters of `parts` CTAs of a kernel the GPU holds at a time (a cluster lies within a part of the chip, so not all SMs can
+// be had).  A property of the kernel and the chip: asked once.
+template <typename K>
+static int clusters_at_a_time(K kernel, int parts, int threads, size_t smem) {
+  struct Known { const void* kernel; int parts, clusters; };
+  static thread_local Known known[128];
+  static thread_local int n_known = 0;
+  for (int i = 0; i < n_known; ++i)
+    if (known[i].kernel == (const void*)kernel && known[i].parts == parts) return known[i].clusters;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(parts * 148));
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr;
+  attr.id = cudaLaunchAttributeClusterDimension;
+  attr.val.clusterDim.x = (unsigned)parts;
+  attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+  cfg.attrs = &attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();
+    n = 0;
+  }
+  if (n_known < 128) known[n_known++] = {(const void*)kernel, parts, n};
+  return n;
+}
+
 // Launches `kernel` over the tiles, their kv heads and parts (x in this order, parts fastest: the tiles with the most keys of
 // every head start first), a tile's parts as a cluster.
 template <typename K, typename... Maps>

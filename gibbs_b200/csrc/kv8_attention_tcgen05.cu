@@ -677,31 +677,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
 
 constexpr int MAX_SHARES = 8;
 
-// How many clusters of `parts` CTAs the GPU holds at a time (a cluster lies within a part of the chip, so not all SMs can be had).
-template <int HD>
-int clusters_at_a_time(int parts) {
-  static int known[MAX_SHARES + 1] = {};                       // (a property of the kernel and the chip)
-  if (known[parts] == 0) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)(parts * 148));
-    cfg.blockDim = dim3(THREADS);
-    cfg.dynamicSmemBytes = Cfg<HD>::SMEM;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)parts;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    int n = 0;
-    if (cudaOccupancyMaxActiveClusters(&n, kv8_attention_tcgen05_kernel<HD>, &cfg) != cudaSuccess) {
-      cudaGetLastError();
-      n = 0;
-    }
-    known[parts] = n > 0 ? n : -1;
-  }
-  return known[parts];
-}
-
 template <int HD>
 int launch(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
   static bool attr_set = false;
@@ -716,7 +691,7 @@ int launch(const Attn& p, long long tiles, long long keys, cudaStream_t stream) 
   const long long most = (keys + KEYS - 1) / KEYS / 4;
   int parts = 1;
   for (int x = 2; x <= MAX_SHARES && x <= most; ++x)
-    if (walks <= clusters_at_a_time<HD>(x)) parts = x;
+    if (walks <= clusters_at_a_time(kv8_attention_tcgen05_kernel<HD>, x, THREADS, Cfg<HD>::SMEM)) parts = x;
   return launch_parts(kv8_attention_tcgen05_kernel<HD>, p, parts, tiles, THREADS, Cfg<HD>::SMEM, stream);
 }
 
