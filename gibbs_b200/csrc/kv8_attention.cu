@@ -249,6 +249,157 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
   join<T, RT, NW>(p, t, kvh, part, parts, m_s, l_s, o_s);
 }
 
+// ---------------------------------------------------------------- heads of 32, 64 or 128 in 32-bit arithmetic
+// The 32-bit path (and bfloat16 heads that the kernels below do not take).  Tiles of 4 rows; a warp takes chunks of 32 keys.  HD / 8
+// lanes share a key, eight bytes each, of K and of V alike, so all loads of a chunk are whole lines and go out together.  A lane's
+// partial scores of its keys are added and handed out in one go (each step exchanges half of them), and end as the scores of ONE key
+// in every lane; weights go back through shared memory.  Bound by FMAs: 2 HD 4 of them for a key.
+template <typename T, int HD>
+__global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
+  constexpr int RT = 4, NW = 4, LPR = HD / 8, KG = 32 / LPR, KEYS = 32 / KG;       // lanes of a key, keys at a time, keys of a lane
+  extern __shared__ __align__(16) float sm[];
+  pdl_trigger();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, db = lane % LPR, kg = lane / LPR;
+  const int part = (int)blockIdx.x % p.parts, unit = (int)blockIdx.x / p.parts, kvh = unit % p.kv_heads;
+  Tile t;
+  if (!find_tile<RT>(p, unit / p.kv_heads, t)) return;         // (the same for every CTA of a cluster)
+  const int c_lo = t.lo / 32, chunks = (t.hi + 31) / 32 - c_lo;
+  const int parts = max(1, min(p.parts, (chunks + NW - 1) / NW));
+  if (part >= parts) return;                                   // (a thread that has left counts as arrived at the cluster's barriers)
+  float* m_s = sm;                                             // [NW + 1][RT], [RT] sums of the CTA
+  float* l_s = m_s + (NW + 2) * RT;                            // [NW][RT]
+  float* o_s = l_s + NW * RT;                                  // [NW][RT][HD]
+  float4* pw = reinterpret_cast<float4*>(o_s + NW * RT * HD) + warp * 32;          // [32] weights of a key
+  pdl_wait();
+  float q[RT][8], o[RT][8], m[RT], l[RT];
+  int pos[RT];
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    m[r] = -INFINITY;
+    l[r] = 0.f;
+    pos[r] = r < t.rows ? t.pos(r) : -1;                       // (a row that does not exist sees nothing)
+    const int tok = (t.row0 + r) / t.group, g = (t.row0 + r) - tok * t.group;
+    const T* src = reinterpret_cast<const T*>(p.q) + (size_t)(t.qstart + tok) * p.ldq + (size_t)(kvh * t.group + g) * HD + db * 8;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      q[r][e] = r < t.rows ? to_f32(src[e]) : 0.f;
+      o[r][e] = 0.f;
+    }
+  }
+  const int* bt = p.block_table + (size_t)t.r * p.bt_stride;
+  // The key whose scores end in this lane: at step `b` of the hand-out (LPR / 2, ..., 1) a lane keeps the upper half of its keys where
+  // the bit of its place is set.
+  int own = 0;
+#pragma unroll
+  for (int b = LPR / 2, half = KEYS / 2; b > 0; b >>= 1, half >>= 1) own += (db & b) ? half : 0;
+  const int own_key = own * KG + kg;                           // of a chunk: a lane's keys are kg, kg + KG, ...
+  for (int c = part * NW + warp; c < chunks; c += parts * NW) {
+    // lane = key of the chunk: where its row lies (-1: not visible to any row)
+    const int j = (c_lo + c) * 32 + lane;
+    long long row = -1;
+    float ks = 0.f, vs = 0.f;
+    if (j >= t.lo && j < t.hi) {
+      const int page = bt[j / p.page_size];
+      if (page >= 0 && page < p.n_pages) {
+        const size_t ph = (size_t)page * p.kv_heads + kvh;
+        row = ((long long)ph * p.page_size + j % p.page_size) * HD;
+        ks = fabsf(p.k_scales[ph]) * p.scale_log2;
+        vs = fabsf(p.v_scales[ph]);
+      } else {
+        atomicExch(p.status, STATUS_BAD_PAGE_READ);
+      }
+    }
+    uint2 kw[KEYS], vw[KEYS];
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const long long at = __shfl_sync(0xffffffffu, row, i * KG + kg);
+      kw[i] = vw[i] = make_uint2(0u, 0u);
+      if (at >= 0) {
+        kw[i] = *reinterpret_cast<const uint2*>(p.k_pages + at + db * 8);
+        vw[i] = *reinterpret_cast<const uint2*>(p.v_pages + at + db * 8);
+      }
+    }
+    float s[KEYS][RT];
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      float k[8];
+      unpack8(kw[i], k);
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        s[i][r] = q[r][0] * k[0];
+#pragma unroll
+        for (int e = 1; e < 8; ++e) s[i][r] = fmaf(q[r][e], k[e], s[i][r]);
+      }
+    }
+#pragma unroll
+    for (int b = LPR / 2, half = KEYS / 2; b > 0; b >>= 1, half >>= 1) {
+      const bool upper = (db & b) != 0;
+#pragma unroll
+      for (int i = 0; i < half; ++i)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float keep = upper ? s[i + half][r] : s[i][r], give = upper ? s[i][r] : s[i + half][r];
+          s[i][r] = keep + __shfl_xor_sync(0xffffffffu, give, b);
+        }
+    }
+    // this lane's key: its page's scales, and whether there is one, from the lane that looked it up
+    const float ks_own = __shfl_sync(0xffffffffu, ks, own_key), vs_own = __shfl_sync(0xffffffffu, vs, own_key);
+    const int j_own = (c_lo + c) * 32 + own_key;
+    const bool there = ks_own != 0.f;
+    float w[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const bool seen = there && j_own <= pos[r] && (p.window <= 0 || j_own + p.window > pos[r]);
+      const float v = seen ? s[0][r] * ks_own : -INFINITY;
+      const float top = fmaxf(m[r], warp_max(v));
+      const float use = top == -INFINITY ? 0.f : top;
+      const float corr = exp2f(m[r] - use);                    // (0 when nothing was seen before)
+      const float e = seen ? exp2f(v - use) : 0.f;
+      l[r] = l[r] * corr + e;
+      m[r] = top;
+      w[r] = seen ? e * vs_own : -1.f;                         // -1: this row does not see the key, whatever its value is
+      if (corr != 1.f) {
+#pragma unroll
+        for (int d = 0; d < 8; ++d) o[r][d] *= corr;
+      }
+    }
+    __syncwarp();
+    pw[own_key] = make_float4(w[0], w[1], w[2], w[3]);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < KEYS; ++i) {
+      const float4 a = pw[i * KG + kg];
+      const float wr[RT] = {a.x, a.y, a.z, a.w};
+      float v[8];
+      unpack8(vw[i], v);
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+        if (!(wr[r] < 0.f)) {
+#pragma unroll
+          for (int d = 0; d < 8; ++d) o[r][d] = fmaf(wr[r], v[d], o[r][d]);
+        }
+    }
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    const float sum = warp_sum(l[r]);
+    if (lane == 0) {
+      m_s[warp * RT + r] = m[r];
+      l_s[warp * RT + r] = sum;
+    }
+#pragma unroll
+    for (int d = 0; d < 8; ++d)
+#pragma unroll
+      for (int x = LPR; x < 32; x <<= 1) o[r][d] += __shfl_xor_sync(0xffffffffu, o[r][d], x);
+    if (kg == 0) {
+      float4* at = reinterpret_cast<float4*>(o_s + ((size_t)warp * RT + r) * HD + db * 8);
+      at[0] = make_float4(o[r][0], o[r][1], o[r][2], o[r][3]);
+      at[1] = make_float4(o[r][4], o[r][5], o[r][6], o[r][7]);
+    }
+  }
+  join<T, RT, NW>(p, t, kvh, part, parts, m_s, l_s, o_s);
+}
+
 // ---------------------------------------------------------------- bfloat16 rows on mma.sync
 // Tiles of 8 NB rows.  K and V stay in 8 bits until they are operands: a lane reads the bytes of its mma fragments and turns two
 // of them at a time into f16, which holds every e4m3 number exactly.  The products are S^T = K Q^T and O^T = V^T P^T: keys (and columns
@@ -682,8 +833,24 @@ int launch_any(const Attn& p, long long tiles, long long keys, cudaStream_t stre
   return launch_parts(kv8_attention_any_kernel<T, NP>, p, key_parts(tiles * p.kv_heads, 148 * 4, (keys + 31) / 32, NW), tiles, 32 * NW,
                       smem, stream);
 }
+template <typename T, int HD>
+int launch_rows(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
+  constexpr int RT = 4, NW = 4, SMEM = ((2 * NW + 2) * RT + NW * RT * HD) * 4 + NW * 32 * 16;
+  static bool attr_set = false;
+  if (!attr_set) {
+    GB_CUDA(cudaFuncSetAttribute(kv8_attention_rows_kernel<T, HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
+    attr_set = true;
+  }
+  return launch_parts(kv8_attention_rows_kernel<T, HD>, p, key_parts(tiles * p.kv_heads, 148 * 3, (keys + 31) / 32, NW), tiles, 32 * NW, SMEM,
+                      stream);
+}
 template <typename T>
 int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
+  switch (p.hd) {
+    case 32: return launch_rows<T, 32>(p, tiles, keys, stream);
+    case 64: return launch_rows<T, 64>(p, tiles, keys, stream);
+    case 128: return launch_rows<T, 128>(p, tiles, keys, stream);
+  }
   switch ((p.hd + 63) / 64) {
     case 1: return launch_any<T, 1>(p, tiles, keys, stream);
     case 2: return launch_any<T, 2>(p, tiles, keys, stream);
