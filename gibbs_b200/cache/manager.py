@@ -19,6 +19,14 @@ Two kinds of memory, both sized once at start:
   needs some, as byte ranges of one row; a slot is zeroed when a request
   takes it.
 
+A request can be forked (``fork``): a second one then stands where it stands.
+Pages that are full are shared, held by both and never written again; the page
+that both would go on writing, and the slot, are copied.
+
+With ``kv_dtype`` float8_e4m3fn the keys and values of mixers that can read
+them so lie in 8-bit pages, with a float32 scale for each page and kv head
+beside them (``ops.kv8``).
+
 The manager is plain host code apart from the tensors it allocates, so its
 bookkeeping runs (and is tested) without a GPU.
 """
@@ -52,6 +60,7 @@ class PagedKVView:
     window: Optional[int]
     block: Optional[int] = None        # the pages keep the current block of this many positions
     keep_first: int = 0                # beside a window: the first positions of a sequence stay as well
+    in_8_bits: Optional[object] = None # the pages with their scales (ops.kv8.Pages), where the cache is held in 8 bits
 
 
 @dataclass
@@ -93,7 +102,7 @@ class CacheManager:
     GUARD_BYTE = 0x5A
 
     def __init__(self, entry_needs, n_pages, page_size: int, n_slots: int, dtype: torch.dtype, device,
-                 max_context: int, guard: bool = False):
+                 max_context: int, guard: bool = False, kv_dtype: Optional[torch.dtype] = None):
         """entry_needs: for each entry of the model's order, (list of needs,
         entry whose cache it reads instead or None).  n_pages: an int (for
         every group) or a dict from retention rule (None = all keys, a window
@@ -101,7 +110,19 @@ class CacheManager:
         ``guard``: one page before and after every page tensor, one slot row
         before and after the slots and 16 bytes behind every slot are filled
         with a pattern that ``check`` looks at: a kernel that writes outside
-        the page or slot it was given is then found where it happened."""
+        the page or slot it was given is then found where it happened.
+        ``kv_dtype``: what keys and values are held in, ``dtype`` (None) or
+        float8_e4m3fn, which every mixer with keys and values has to take."""
+        if kv_dtype not in (None, dtype, torch.float8_e4m3fn):
+            raise ValueError(f"keys and values are held in {dtype} or in float8_e4m3fn, not in {kv_dtype}")
+        self.in_8_bits = kv_dtype == torch.float8_e4m3fn
+        if self.in_8_bits:
+            keyed = [(e, need) for e, (needs, reads) in enumerate(entry_needs) if reads is None for need in needs
+                     if isinstance(need, PagedKV)]
+            refused = [e for e, need in keyed if not need.in_8_bits]
+            if refused or not keyed:
+                raise ValueError("an 8-bit cache: " + (f"the mixers of entries {refused} do not take keys and values in 8 bits"
+                                                       if keyed else "the model has no layer with keys and values"))
         if page_size <= 0:
             raise ValueError(f"page_size {page_size}")
         self.page_size, self.n_slots, self.dtype = page_size, n_slots, dtype
@@ -114,6 +135,7 @@ class CacheManager:
         self.groups: list[_Group] = []
         self._group_of: dict[tuple[int, int], int] = {}
         self._pages: dict[tuple[int, int], tuple[torch.Tensor, torch.Tensor]] = {}
+        self._scaled: dict = {}                     # with ``in_8_bits``: (entry, need) -> ops.kv8.Pages
         self._slot_ranges: dict[tuple[int, int], tuple[int, int, SlotState]] = {}
         slot_bytes = 0
         by_window: dict = {}
@@ -137,6 +159,12 @@ class CacheManager:
                                                                  dtype), None)
                         continue
                     shape = (self.groups[g].pool.size, need.kv_heads, page_size)
+                    if self.in_8_bits:
+                        from ..ops import kv8
+                        kp, vp = (self._page_tensor(shape + (need.head_dim,), kv8.DTYPE) for _ in range(2))
+                        self._pages[(e, k)] = (kp, vp)
+                        self._scaled[(e, k)] = kv8.Pages(kp, vp, *(self._page_tensor(shape[:2], torch.float32) for _ in range(2)))
+                        continue
                     self._pages[(e, k)] = (self._page_tensor(shape + (need.head_dim,), dtype),
                                            self._page_tensor(shape + (need.value_dim,), dtype))
                 elif isinstance(need, SlotState):
@@ -190,7 +218,7 @@ class CacheManager:
                 total += kp.shape[2] * kp.element_size()
             else:
                 total += kp.shape[1] * (kp.shape[3] + vp.shape[3]) * kp.element_size()
-        return total
+        return total                                # (8-bit pages have 8 bytes of scales a page and head besides)
 
     def pages_needed(self, length: int) -> int:
         return -(-length // self.page_size)
@@ -233,10 +261,17 @@ class CacheManager:
         (request cache, new length), once every request of the list has given
         back the pages its window has passed."""
         need = [0] * len(self.groups)
+        given: dict = {}                            # (group, shared page) -> holders that will give it back
         for rc, new_length in wants:
             for g, group in enumerate(self.groups):
                 table = rc.block_tables[g]
-                freed = sum(1 for i in self._passed_pages(group, rc.length, table) if table[i] >= 0)
+                passed = [table[i] for i in self._passed_pages(group, rc.length, table) if table[i] >= 0]
+                freed = len(passed)
+                if group.pool.n_shared:
+                    freed = 0                       # a shared page is free when its last holder gives it back
+                    for p in passed:
+                        given[(g, p)] = given.get((g, p), 0) + 1
+                        freed += given[(g, p)] == group.pool.holders(p)
                 need[g] += max(self.pages_needed(new_length) - len(table), 0) - freed
         return need
 
@@ -309,13 +344,70 @@ class CacheManager:
             self.slots.give_back(rc.slot)
             rc.slot = None
 
+    def fork(self, parent_id, child_id) -> list:
+        """A new request that stands where ``parent_id`` stands: full pages are shared, the page that both will go on writing
+        and the state slot are the child's own.  Returns what has to be copied before either is stepped again: for each list
+        of ``copied_tensors`` the (source, destination) rows.  All or nothing: raises OutOfSlots or OutOfPages and takes
+        nothing when there is no slot or page."""
+        parent = self.live.get(parent_id)
+        if parent is None:
+            raise PoolError(f"request {parent_id!r} is not live")
+        if child_id in self.live:
+            raise PoolError(f"request {child_id!r} is already live")
+        held, full = self.pages_needed(parent.length), parent.length // self.page_size
+        short = [g for g, group in enumerate(self.groups)
+                 if held > full and parent.block_tables[g][full] >= 0 and group.pool.n_free == 0]
+        if short:
+            raise OutOfPages(f"no page to fork request {parent_id!r}: groups {short} have none free")
+        slot = None
+        if self.slot_bytes:
+            slot = self.slots.take()
+            if slot is None:
+                raise OutOfSlots(f"all {self.n_slots} state slots are in use")
+        tables, pairs = [], []
+        for g, group in enumerate(self.groups):
+            table, copies = [], []
+            for i, page in enumerate(parent.block_tables[g][:held]):
+                if page < 0:
+                    table.append(-1)
+                elif i < full:
+                    table.append(group.pool.share(page))
+                else:
+                    table.append(group.pool.take())
+                    copies.append((page, table[-1]))
+            tables.append(table)
+            pairs.append(copies)
+        if self.slot_bytes:
+            pairs.append([(parent.slot, slot)])
+        self.live[child_id] = RequestCache(child_id, slot, tables, parent.length)
+        return pairs
+
+    def copied_tensors(self) -> list:
+        """The tensors whose rows a fork copies: for each group those that its page ids address (with the scales of 8-bit
+        pages), and behind them, where there are slots, the slots' memory."""
+        out = [[] for _ in self.groups]
+        for key, (kp, vp) in self._pages.items():
+            if key in self._scaled:
+                out[self._group_of[key]] += list(self._scaled[key].tensors())
+            else:
+                out[self._group_of[key]] += [kp] if vp is None else [kp, vp]
+        return out + ([[self._slot_mem]] if self.slot_bytes else [])
+
     def check(self) -> None:
-        """Invariants: no page or slot lost, none held twice."""
+        """Invariants: no page or slot lost, none held by more than it counts, and none that is shared still to be written."""
         for g, group in enumerate(self.groups):
             group.pool.check()
-            held = [p for rc in self.live.values() for p in rc.block_tables[g] if p >= 0]
-            if len(held) != len(set(held)):
-                raise PoolError(f"a page of group {g} is held twice")
+            held: dict = {}
+            for rc in self.live.values():
+                for i, p in enumerate(rc.block_tables[g]):
+                    if p >= 0:
+                        held.setdefault(p, []).append((rc, i))
+            for p, by in held.items():
+                if len(by) != group.pool.holders(p):
+                    raise PoolError(f"a page of group {g} is held twice" if len(by) > group.pool.holders(p) else
+                                    f"group {g}: page {p} has {group.pool.holders(p)} holders, requests hold it {len(by)} times")
+                if len(by) > 1 and any((i + 1) * self.page_size > rc.length for rc, i in by):
+                    raise PoolError(f"group {g}: page {p} is shared and not full")
             if len(held) != group.pool.n_used:
                 raise PoolError(f"group {g}: {group.pool.n_used} pages are out but requests hold {len(held)}")
         self.slots.check()
@@ -354,7 +446,7 @@ class CacheManager:
                     kp, vp = self._pages[(owner, k)]
                     g = self._group_of[(owner, k)]
                     views.append(PagedKVView(kp, vp, block_tables[g], self.page_size, reads is None, need.window, need.block,
-                                             int(getattr(need, "keep_first", 0) or 0)))
+                                             int(getattr(need, "keep_first", 0) or 0), self._scaled.get((owner, k))))
                 else:
                     views.append(SlotView(self._slot_views[(owner, k)], slot_ids, host_slot_ids))
             out.append(views)

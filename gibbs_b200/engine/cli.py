@@ -35,6 +35,8 @@ def build_parser() -> argparse.ArgumentParser:
     ap.add_argument("--top-k", type=int, default=50, help="1..64, default 50; 0: off (the sampler's 64 candidates, narrowed by --top-p only)")
     ap.add_argument("--seed", type=int, default=None, help="sampling seed; also the seed of --random")
     ap.add_argument("--dtype", default="bfloat16", choices=["bfloat16", "float32"])
+    ap.add_argument("--cache-dtype", default=None, choices=["float8_e4m3"],
+                    help="hold keys and values in 8 bits (default: in the compute dtype)")
     ap.add_argument("--page-size", type=int, default=16)
     ap.add_argument("--max-batch-tokens", type=int, default=2048)
     ap.add_argument("--bench", help="suite.json: {defaults: {...}, models: [{id: DIR, ...}]}; one JSON line per model")
@@ -97,7 +99,8 @@ def bench_suite(path: Path, a) -> int:
         batch = int(m.get("batch", defaults.get("batch", 1)))
         ctx = a.ctx or prefill_tokens + decode_tokens + 64
         gen = Generator(folder, dtype=a.dtype, device=a.device, ctx=ctx, page_size=a.page_size,
-                        max_running=max(batch, 1), max_batch_tokens=max(a.max_batch_tokens, prefill_tokens))
+                        max_running=max(batch, 1), max_batch_tokens=max(a.max_batch_tokens, prefill_tokens),
+                        cache_dtype=a.cache_dtype)
         pre = B.measure_prefill(gen.engine, prefill_tokens, warmup=3, runs=runs)
         decs = [B.measure_decode(gen.engine, batch, prefill_tokens, decode_tokens, 3, seed=r) for r in range(runs)]
         dec = sorted(decs, key=lambda d: d["tok_s"])[len(decs) // 2]
@@ -142,7 +145,7 @@ def main(argv=None) -> int:
     from .api import Generator
     from .step import StepEntry
     gen = Generator(folder, dtype=a.dtype, device=a.device, ctx=a.ctx, page_size=a.page_size, max_running=4,
-                    max_batch_tokens=a.max_batch_tokens, seed=a.seed or 0, arch=a.arch)
+                    max_batch_tokens=a.max_batch_tokens, seed=a.seed or 0, arch=a.arch, cache_dtype=a.cache_dtype)
     if a.probe_top5:
         ids = _ids(a.probe_top5)
         gen.engine.open("probe")

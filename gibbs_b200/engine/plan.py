@@ -286,6 +286,34 @@ class PlanBuilder:
                                 ops.dtype_code(out.dtype), bt_stride], [scale, softcap], label="attention")
         return out
 
+    def kv8_store(self, qkv: torch.Tensor, heads: int, kv_heads: int, hd: int, q_gain, k_gain, eps: float, rotary, kv_view,
+                  write_kv: bool) -> torch.Tensor:
+        """Norm and rotation of q and k, k and v into 8-bit pages; returns the rotated q.  Takes the partial tiles of the
+        product in front."""
+        from ..ops import kv8
+        if not isinstance(kv_view.block_table, TableRef):
+            raise NotPlannable("attention reads the step's block tables")
+        pages = kv_view.in_8_bits
+        q_out = self.buffer("q_rotated", heads * hd)
+        cache = [self.keep(t) for t in pages.tensors()] if write_kv else [0, 0, 0, 0]
+        self.emit(kv8.plan_id("kv8_store"),
+                  [qkv.data_ptr(), qkv.stride(0), ops.dtype_code(qkv.dtype), q_out.data_ptr(), self.keep(q_gain), self.keep(k_gain),
+                   self.keep(None if rotary is None else rotary.table), 0 if rotary is None else rotary.rotary_dim,
+                   0 if rotary is None else int(rotary.adjacent_pairs), *cache, pages.n_pages if write_kv else 0, pages.page_size,
+                   heads, kv_heads, hd, sym(S_BLOCK_TABLE0 + kv_view.block_table.group), self.bt_stride], [eps],
+                  flags=kv8.TAKES_PARTIALS, label="kv8_store")
+        return q_out
+
+    def kv8_attention(self, q: torch.Tensor, heads: int, kv_heads: int, hd: int, scale: float, window: int, kv_view) -> torch.Tensor:
+        from ..ops import kv8
+        pages = kv_view.in_8_bits
+        out = self.buffer("mixed", heads * hd)
+        self.emit(kv8.plan_id("kv8_attention"),
+                  [q.data_ptr(), q.stride(0), ops.dtype_code(q.dtype), out.data_ptr(), out.stride(0),
+                   *[self.keep(t) for t in pages.tensors()], pages.n_pages, pages.page_size, heads, kv_heads, hd,
+                   sym(S_BLOCK_TABLE0 + kv_view.block_table.group), self.bt_stride, int(window or 0)], [scale], label="kv8_attention")
+        return out
+
     def scale_softcap(self, values: int, columns: int, rows_symbol: int, scale: float, cap: float) -> None:
         """values <- values * scale, then cap * tanh(values / cap) when cap > 0; ``values`` is a
         symbol (the step's logits) or an address, [rows, columns] float32."""

@@ -41,6 +41,14 @@ Ends by length are foreseen and leave the batch on time.  Whenever the next
 step needs the host's decisions first (a request waits for admission, one
 was cancelled, the pages would not suffice), the step in flight is read
 before anything else happens, and the scheduler goes on as without overlap.
+
+Several answers to one prompt (``submit(..., samples=n)``).  The first request
+runs the prompt; the others wait with it, and in the step that ends the prompt
+each takes its first token from the same logits and is forked from the first
+(``Engine.fork``: full pages shared, the last one and the state copied).  When
+some find no slot or page then, or the first is cancelled or fails, the next of
+them runs the prompt again for those that are left; a request's seed and the
+number of tokens it has drawn decide its picks, whoever ran its prompt.
 """
 from __future__ import annotations
 
@@ -127,6 +135,7 @@ class Sequence_:
     admitted: int = -1                              # admission order (for preemption)
     preemptions: int = 0
     cancelled: bool = False
+    followers: list = field(default_factory=list)   # further answers to this prompt that wait for it to have been run
 
     @property
     def tokens(self) -> list:
@@ -215,7 +224,21 @@ class Scheduler:
         self.steps = 0
 
     # -- submission --------------------------------------------------------------
-    def submit(self, prompt: Sequence[int], params: Optional[SamplingParams] = None) -> int:
+    def submit(self, prompt: Sequence[int], params: Optional[SamplingParams] = None, samples: int = 1):
+        """The id of a new request.  ``samples`` > 1: the ids of as many requests for answers to one prompt, which is run
+        once; with ``params.seed`` None each has a seed of its own, otherwise seed, seed + 1, ..."""
+        if samples < 1:
+            raise ValueError(f"{samples} samples")
+        if samples > 1:
+            params = params or SamplingParams()
+            each = [params if params.seed is None else SamplingParams(**{**params.__dict__, "seed": params.seed + i}) for i in range(samples)]
+            ids = [self.submit(prompt, p) for p in each]
+            leader = self.sequences[ids[0]]
+            for sid in ids[1:]:
+                seq = self.sequences[sid]
+                self.waiting.remove(seq)
+                leader.followers.append(seq)
+            return ids
         params = params or SamplingParams()
         prompt = [int(t) for t in prompt] or [1]
         if len(prompt) >= self.ctx:
@@ -247,6 +270,30 @@ class Scheduler:
             self.waiting.remove(seq)
         seq.state, seq.finish, seq.error = SeqState.FINISHED, reason, error
         out.finished.append((seq.id, reason))
+        self._release(seq)
+
+    def _release(self, seq: Sequence_) -> None:
+        """What still waits for this request's prompt: the first of them runs it next, and the others wait for that one (for an
+        engine that cannot fork, every one runs it)."""
+        followers, seq.followers = seq.followers, []
+        live = [f for f in followers if not f.cancelled]
+        if live and hasattr(self.engine, "fork"):
+            live[0].followers = live[1:]
+            live = live[:1]
+        self.waiting.extendleft(reversed(live + [f for f in followers if f.cancelled]))
+
+    def _join(self, leader: Sequence_, follower: Sequence_) -> bool:
+        """Fork ``follower`` from ``leader``, which has just run their prompt; False when it cannot be."""
+        if not hasattr(self.engine, "fork") or follower.cancelled or len(self.running) >= self.max_running:
+            return False
+        try:
+            self.engine.fork(leader.id, follower.id)
+        except (OutOfSlots, OutOfPages):
+            return False
+        follower.state, follower.admitted, follower.fed = SeqState.RUNNING, self._admissions, len(follower.prompt)
+        self._admissions += 1
+        self.running.append(follower)
+        return True
 
     def _preempt(self, seq: Sequence_, out: StepOutput):
         self.engine.close(seq.id)
@@ -364,11 +411,18 @@ class Scheduler:
 
         entries, samplers = [], []
         n_prefill = n_decode = 0
+        room = getattr(self.engine, "max_step_tokens", 1 << 30) - len(plan)      # rows of logits beside one for every request
+        joined = False
         for s, n in plan:
             last = s.fed + n == len(s.prompt) + len(s.output)
-            entries.append(StepEntry(s.id, s.span(s.fed, s.fed + n), [n - 1] if last else []))
+            # (the same logits once more for every request that waits for this prompt)
+            take = s.followers[:max(0, min(room, self.max_running - 1))] if last and not s.output else []
+            room -= len(take)
+            joined = joined or bool(take)
+            entries.append(StepEntry(s.id, s.span(s.fed, s.fed + n), [n - 1] * (1 + len(take)) if last else []))
             if last:
                 samplers.append(s)
+                samplers += take
             if s.decoding:
                 n_decode += 1
             else:
@@ -377,7 +431,7 @@ class Scheduler:
         # (and none only ran to fill its cache, max_new_tokens == 0)
         # and nobody asks what the distribution said about its token: that is read from the logits at once)
         # (nor has a repetition penalty, which needs every token so far on the host)
-        lag = self.overlap and len(samplers) == len(plan) and all(
+        lag = self.overlap and not joined and len(samplers) == len(plan) and all(
             s.params.max_new_tokens > 0 and s.params.top_logprobs is None and not s.params.penalizes
             for s in samplers)
         t0 = self.clock()
@@ -404,6 +458,11 @@ class Scheduler:
             return out
         for s, n in plan:
             s.fed += n
+            if s.followers and s.fed >= len(s.prompt):
+                picks = [f for f in s.followers if any(f is x for x in samplers)]
+                kept = [f for f in picks if self._join(s, f)]
+                s.followers = [f for f in s.followers if not any(f is x for x in kept)]
+                self._release(s)                    # (those that found no place; their token is picked again)
         if pending is not None:
             self._inflight = _InFlight(samplers, pending, t0, n_prefill, n_decode)
             out.active_sequences = len(self.running)
@@ -513,10 +572,11 @@ class Scheduler:
             outs.append(self.step())
         return outs
 
-    def generate(self, prompts: Sequence[Sequence[int]], params=None) -> list:
-        """Submit prompts, run to the end, return each one's generated ids."""
+    def generate(self, prompts: Sequence[Sequence[int]], params=None, samples: int = 1) -> list:
+        """Submit prompts, run to the end, return each one's generated ids (``samples`` > 1: a list of as many answers)."""
         if params is None or isinstance(params, SamplingParams):
             params = [params] * len(prompts)
-        ids = [self.submit(p, q) for p, q in zip(prompts, params)]
+        ids = [self.submit(p, q, samples) for p, q in zip(prompts, params)]
         self.run()
-        return [list(self.sequences[i].output) for i in ids]
+        answer = lambda i: list(self.sequences[i].output)                                              # noqa: E731
+        return [answer(i) if samples == 1 else [answer(j) for j in i] for i in ids]

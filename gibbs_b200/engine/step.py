@@ -178,13 +178,28 @@ class StepBuilder:
         return step, caches
 
 
+_CACHE_DTYPES = {"float8_e4m3": torch.float8_e4m3fn, "float8_e4m3fn": torch.float8_e4m3fn, "fp8": torch.float8_e4m3fn}
+
+
+def parse_cache_dtype(name) -> Optional[torch.dtype]:
+    """What keys and values are held in: None (the compute dtype) or float8_e4m3fn."""
+    if name is None or name == torch.float8_e4m3fn:
+        return name
+    try:
+        return _CACHE_DTYPES[str(name).lower()]
+    except KeyError:
+        raise ValueError(f"unknown cache dtype '{name}'; use float8_e4m3, or none for the compute dtype") from None
+
+
 class Engine:
     """A model, its cache and the step function over them."""
 
     def __init__(self, model: CausalLM, n_pages: int, page_size: int = 16, max_requests: int = 64,
                  max_step_tokens: int = 8192, max_context: Optional[int] = None, use_graphs: bool = True,
-                 use_plan: bool = True, guard_cache: bool = False, timing: Optional[bool] = None):
-        """``timing`` (default: the environment variable GIBBS_B200_TIMING=1): every operation of
+                 use_plan: bool = True, guard_cache: bool = False, timing: Optional[bool] = None, cache_dtype=None):
+        """``cache_dtype``: what keys and values are held in: the compute dtype (None), or 8 bits ("float8_e4m3"), for models
+        whose attention layers take it.
+        ``timing`` (default: the environment variable GIBBS_B200_TIMING=1): every operation of
         a step is timed with CUDA events and added up per kind (``timing_table``); steps then run
         without CUDA graphs and their kernels do not overlap."""
         self.model = model
@@ -194,8 +209,12 @@ class Engine:
         ops.ensure_built(sorted(model.kernel_libraries()))
         self.max_context = int(max_context or model.plan.max_context)
         self.max_requests, self.max_step_tokens = int(max_requests), int(max_step_tokens)
+        kv_dtype = parse_cache_dtype(cache_dtype)
+        if kv_dtype is not None:
+            ops.ensure_built(["kv8"])
         self.cache = CacheManager(model.entry_needs(), n_pages, page_size, self.max_requests, model.rt.dtype,
-                                  self.device, self.max_context, guard=guard_cache)
+                                  self.device, self.max_context, guard=guard_cache, kv_dtype=kv_dtype)
+        self._row_copies = None
         self.vocab_size = model.vocab_size
         self.status = ops.device_status(self.device)
         self.builder = StepBuilder(self.cache, self.device, self.max_requests, self.max_step_tokens, self.status)
@@ -236,6 +255,21 @@ class Engine:
 
     def close(self, request_id) -> None:
         self.cache.close(request_id)
+
+    def fork(self, request_id, new_id) -> None:
+        """Open ``new_id`` where ``request_id`` stands: both go on from the same tokens, each on its own.  Full pages are
+        shared; the page that both will write on and the state of layers that keep some are copied, in one launch.  Raises
+        OutOfPages or OutOfSlots, and changes nothing, when the pools cannot hold the new request."""
+        if self._row_copies is None:
+            tensors = self.cache.copied_tensors()
+            self._row_copies = ops.RowCopies(tensors) if tensors else False
+        pairs = self.cache.fork(request_id, new_id)
+        try:
+            if self._row_copies and any(pairs):
+                self._row_copies.copy(pairs)
+        except BaseException:
+            self.cache.close(new_id)
+            raise
 
     def length(self, request_id) -> int:
         return self.cache.live[request_id].length
@@ -293,6 +327,9 @@ class Engine:
             raise StepError(f"{len(entries)} requests in one step; the engine was made for {self.max_requests}")
         if total > self.max_step_tokens:
             raise StepError(f"{total} tokens in one step; the engine was made for {self.max_step_tokens}")
+        wanted = sum(len(e.want) for e in entries)                  # (a place may be wanted more than once)
+        if wanted > self.max_step_tokens:
+            raise StepError(f"{wanted} rows of logits wanted in one step; the engine was made for {self.max_step_tokens}")
         return total, arrays
 
     def step(self, entries: Sequence[StepEntry], feed=None) -> Optional[torch.Tensor]:

@@ -7,12 +7,15 @@ the residual stream (MisterTK/gibbs arch/lib/transformer.json5:46-87;
 src/graph/cpu.rs:826-951).  ``window`` keeps the last ``window`` keys visible
 only; ``shares_kv`` makes the layer read a cache another entry writes: it
 then has no k/v projections of its own (transformer.json5:39-41, write: false).
+Keys and values may be held in 8 bits (``ops.kv8``): the norm, the rotation and
+the formula are the same, on what the pages stand for.
 """
 from __future__ import annotations
 
 import torch
 
 from .. import ops
+from ..ops import kv8
 from .base import Mixer, PagedKV, TensorDecl, VECTOR, part_class, register_part
 from .linear import Linear
 
@@ -72,7 +75,9 @@ class GQAAttention(Mixer):
         return tuple(set(self.qkv.kernel_libraries()) | set(self.out_proj.kernel_libraries()) | {"core"})
 
     def cache_needs(self):
-        return [] if self.shares_kv else [PagedKV(self.kv_heads, self.head_dim, self.window)]
+        # (in 8 bits: without a soft cap, and heads that the kernels hold)
+        in_8_bits = self.softcap <= 0 and self.head_dim % 8 == 0 and self.head_dim <= kv8.MAX_HEAD_DIM
+        return [] if self.shares_kv else [PagedKV(self.kv_heads, self.head_dim, self.window, in_8_bits=in_8_bits)]
 
     def attention_flops(self, n_tokens: int) -> int:
         """Scores and weighted values of a whole prompt over the causal half (or the
@@ -92,6 +97,14 @@ class GQAAttention(Mixer):
                 False if rot is None else rot.adjacent_pairs)
         pages = (None if self.shares_kv else kv.k_pages, None if self.shares_kv else kv.v_pages)
         a = self.heads * self.head_dim
+        if kv.in_8_bits is not None:
+            self._takes_8_bits()
+            q = kv8.qk_norm_rope_store(qkv, self.rt.empty(qkv.shape[0], a), self.heads, self.kv_heads, self.head_dim, self.q_gain,
+                                       self.k_gain, self.eps, *rope, step, kv.block_table, None if self.shares_kv else kv.in_8_bits)
+            out = kv8.paged_attention(q, self.heads, self.kv_heads, self.head_dim, kv.in_8_bits, kv.block_table, self.scale,
+                                      self.window or 0, self.rt.empty(qkv.shape[0], a), step)
+            self.out_proj(out, out=residual, accumulate=True)
+            return
         if isinstance(qkv, ops.Partials):
             # K was split: this kernel adds the partial tiles itself (no reduction kernel in between)
             q = ops.qk_norm_rope_store_partials(
@@ -107,12 +120,24 @@ class GQAAttention(Mixer):
                             step.status, hints=step, softcap=self.softcap)
         self.out_proj(out, out=residual, accumulate=True)
 
+    def _takes_8_bits(self) -> None:
+        """(A layer that reads another's cache asks for none itself, so it is looked at here.)"""
+        if self.softcap > 0:
+            raise ops.KernelError("attention with a soft cap on its scores does not take an 8-bit cache")
+
     def plan_ops(self, plan, h, caches):
         kv = caches[0]
         if not self.shares_kv and not kv.writable:
             raise RuntimeError("an attention layer with k/v projections was given a read-only cache")
         qkv = plan.linear(h, self.qkv.weight, self.qkv.bias, plan.buffer("qkv", self.qkv.out_features), "plain",
                           partials="always", role="qkv")
+        if kv.in_8_bits is not None:
+            self._takes_8_bits()
+            q = plan.kv8_store(qkv, self.heads, self.kv_heads, self.head_dim, self.q_gain, self.k_gain, self.eps, self.rotary, kv,
+                               not self.shares_kv)
+            out = plan.kv8_attention(q, self.heads, self.kv_heads, self.head_dim, self.scale, self.window or 0, kv)
+            plan.linear(out, self.out_proj.weight, self.out_proj.bias, None, "residual", role="out_proj")
+            return
         plan.qk_norm_rope_store(qkv, self.heads, self.kv_heads, self.head_dim, self.q_gain, self.k_gain, self.eps,
                                 self.rotary, kv, not self.shares_kv, plan.bt_stride)
         out = plan.attention(self.heads, self.kv_heads, self.head_dim, self.scale, self.window or 0, kv,

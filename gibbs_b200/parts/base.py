@@ -84,6 +84,8 @@ class PagedKV:
     block: Optional[int] = None
     # with a window: the pages that hold the first ``keep_first`` positions of a sequence stay as well
     keep_first: int = 0
+    # the mixer also works on 8-bit pages with a scale for each page and kv head (ops.kv8)
+    in_8_bits: bool = False
 
     def __post_init__(self):
         if self.window is not None and self.block is not None:
