@@ -100,6 +100,10 @@ static inline Step step_of(const GbPlanCtx* ctx) {
   return s;
 }
 
+// An entry of a block table, for kernels that look at it later: one that is not a page's id is as large as no pool (and never -1,
+// which stands for keys that nobody sees).
+__device__ __forceinline__ int page_id(const int* entry) { return (int)min((unsigned)*entry, 0x7fffffffu); }
+
 // Piece `index` of a launch over pieces of requests, `count(r)` for request r: which request (-1: none) and which of its
 // pieces.  A whole warp looks at 32 requests at a time; every lane gets the answer.  With `last_first` the requests are
 // taken from the last to the first.

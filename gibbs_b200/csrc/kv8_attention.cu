@@ -293,22 +293,33 @@ __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
 #pragma unroll
   for (int b = LPR / 2, half = KEYS / 2; b > 0; b >>= 1, half >>= 1) own += (db & b) ? half : 0;
   const int own_key = own * KG + kg;                           // of a chunk: a lane's keys are kg, kg + KG, ...
-  for (int c = part * NW + warp; c < chunks; c += parts * NW) {
-    // lane = key of the chunk: where its row lies (-1: not visible to any row)
+  // lane = key of a chunk.  What a chunk needs before its loads is asked for ahead: its page's id two chunks ahead, the page's scales
+  // one ahead, so that a chunk waits for one trip and not for three.
+  const int stride = parts * NW;
+  auto page_of = [&](int c) {                                  // -1: not visible to any row
     const int j = (c_lo + c) * 32 + lane;
-    long long row = -1;
-    float ks = 0.f, vs = 0.f;
-    if (j >= t.lo && j < t.hi) {
-      const int page = bt[j / p.page_size];
-      if (page >= 0 && page < p.n_pages) {
-        const size_t ph = (size_t)page * p.kv_heads + kvh;
-        row = ((long long)ph * p.page_size + j % p.page_size) * HD;
-        ks = fabsf(p.k_scales[ph]) * p.scale_log2;
-        vs = fabsf(p.v_scales[ph]);
-      } else {
-        atomicExch(p.status, STATUS_BAD_PAGE_READ);
-      }
+    return (c >= chunks || j < t.lo || j >= t.hi) ? -1 : page_id(bt + j / p.page_size);
+  };
+  long long row_next;
+  float ks_next, vs_next;
+  auto look_up = [&](int c, int page) {
+    row_next = -1;
+    ks_next = vs_next = 0.f;
+    if (page < 0) return;
+    if (page >= p.n_pages) {
+      atomicExch(p.status, STATUS_BAD_PAGE_READ);
+      return;
     }
+    const size_t ph = (size_t)page * p.kv_heads + kvh;
+    row_next = ((long long)ph * p.page_size + ((c_lo + c) * 32 + lane) % p.page_size) * HD;
+    ks_next = p.k_scales[ph];
+    vs_next = p.v_scales[ph];
+  };
+  look_up(part * NW + warp, page_of(part * NW + warp));
+  int page_next = page_of(part * NW + warp + stride);
+  for (int c = part * NW + warp; c < chunks; c += stride) {
+    const long long row = row_next;
+    const float ks = fabsf(ks_next) * p.scale_log2, vs = fabsf(vs_next);       // vs 0: no such key
     uint2 kw[KEYS], vw[KEYS];
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
@@ -319,6 +330,8 @@ __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
         vw[i] = *reinterpret_cast<const uint2*>(p.v_pages + at + db * 8);
       }
     }
+    look_up(c + stride, page_next);
+    page_next = page_of(c + 2 * stride);
     float s[KEYS][RT];
 #pragma unroll
     for (int i = 0; i < KEYS; ++i) {
@@ -345,7 +358,7 @@ __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
     // this lane's key: its page's scales, and whether there is one, from the lane that looked it up
     const float ks_own = __shfl_sync(0xffffffffu, ks, own_key), vs_own = __shfl_sync(0xffffffffu, vs, own_key);
     const int j_own = (c_lo + c) * 32 + own_key;
-    const bool there = ks_own != 0.f;
+    const bool there = vs_own != 0.f;
     float w[RT];
 #pragma unroll
     for (int r = 0; r < RT; ++r) {
@@ -497,7 +510,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   constexpr int NONE = -1;
   auto page_of = [&](int n) {
     const int c = first + (n / NG) * stride, j = (c_lo + c) * CK + (n % NG) * 16;
-    return (c >= chunks || j >= t.hi || j + 15 < t.lo) ? NONE : bt[j >> p.page_shift] & 0x7fffffff;
+    return (c >= chunks || j >= t.hi || j + 15 < t.lo) ? NONE : page_id(bt + (j >> p.page_shift));
   };
   auto checked = [&](int page) {                               // (apart from the lookup, so that its trip is not waited for there)
     if (page < p.n_pages) return page;
@@ -814,10 +827,12 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
 }
 
 // ---------------------------------------------------------------- launches
-// How many CTAs share a tile's keys: as many as fill `slots` places on the GPU, each with a chunk for every warp.
-int key_parts(long long ctas, long long slots, long long chunks, int warps) {
+// How many CTAs share a tile's keys, a chunk for every warp at least: as many as let the chip hold `over` times what is launched.
+template <typename K>
+int parts_that_fit(K kernel, int over, long long ctas, long long chunks, int warps, size_t smem) {
   int parts = 1;
-  while (parts < MAX_PARTS && ctas * parts * 2 <= slots && chunks >= (long long)parts * 2 * warps) parts *= 2;
+  for (int x = 2; x <= MAX_PARTS && chunks > (long long)(x - 1) * warps; ++x)
+    if (ctas <= (long long)over * clusters_at_a_time(kernel, x, 32 * warps, smem)) parts = x;
   return parts;
 }
 
@@ -830,8 +845,8 @@ int launch_any(const Attn& p, long long tiles, long long keys, cudaStream_t stre
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_any_kernel<T, NP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set = true;
   }
-  return launch_parts(kv8_attention_any_kernel<T, NP>, p, key_parts(tiles * p.kv_heads, 148 * 4, (keys + 31) / 32, NW), tiles, 32 * NW,
-                      smem, stream);
+  const int parts = parts_that_fit(kv8_attention_any_kernel<T, NP>, 1, tiles * p.kv_heads, (keys + 31) / 32, NW, smem);
+  return launch_parts(kv8_attention_any_kernel<T, NP>, p, parts, tiles, 32 * NW, smem, stream);
 }
 template <typename T, int HD>
 int launch_rows(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
@@ -841,8 +856,8 @@ int launch_rows(const Attn& p, long long tiles, long long keys, cudaStream_t str
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_rows_kernel<T, HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set = true;
   }
-  return launch_parts(kv8_attention_rows_kernel<T, HD>, p, key_parts(tiles * p.kv_heads, 148 * 3, (keys + 31) / 32, NW), tiles, 32 * NW, SMEM,
-                      stream);
+  const int parts = parts_that_fit(kv8_attention_rows_kernel<T, HD>, 2, tiles * p.kv_heads, (keys + 31) / 32, NW, SMEM);
+  return launch_parts(kv8_attention_rows_kernel<T, HD>, p, parts, tiles, 32 * NW, SMEM, stream);
 }
 template <typename T>
 int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
@@ -881,10 +896,9 @@ int launch_mma_of(const Attn& p, long long tiles, long long keys, cudaStream_t s
   const long long chunks = (keys + C::CK - 1) / C::CK, ctas = tiles * p.kv_heads;
   int parts = 1;
   if (C::CTAS == 1) {
-    for (int x = 2; x <= MAX_PARTS && chunks > (long long)(x - 1) * C::NW; ++x)
-      if (ctas <= clusters_at_a_time(kv8_attention_mma_kernel<HD, NB, WARPS>, x, 32 * C::NW, SMEM)) parts = x;
+    parts = parts_that_fit(kv8_attention_mma_kernel<HD, NB, WARPS>, 1, ctas, chunks, C::NW, SMEM);
   } else {
-    parts = key_parts(ctas, 148 * C::CTAS, chunks, C::NW);
+    while (parts < MAX_PARTS && ctas * parts * 2 <= 148 * C::CTAS && chunks >= (long long)parts * 2 * C::NW) parts *= 2;
   }
   return launch_parts(kv8_attention_mma_kernel<HD, NB, WARPS>, p, parts, tiles, 32 * C::NW, SMEM, stream, mk, mv);
 }
@@ -920,7 +934,7 @@ GB_OP(gb_op_kv8_attention) {
   p.hd = (int)a[13];
   p.block_table = reinterpret_cast<const int*>(a[14]);
   p.bt_stride = (int)a[15];
-  p.window = (int)a[16];
+  p.window = a[16] > 0x3fffffff ? 0 : (int)a[16];               // (one that no context reaches is none, and sums with it stay in 32 bits)
   p.scale_log2 = (float)(f[0] * 1.4426950408889634);
   p.status = ctx->status;
   if (p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads != 0 || p.hd <= 0 || p.hd % 8 != 0 || p.hd > 256 || p.page_size <= 0)

@@ -67,11 +67,11 @@ static bool group_map(CUtensorMap* map, const void* pages, long long rows, int h
 // be had).  A property of the kernel and the chip: asked once.
 template <typename K>
 static int clusters_at_a_time(K kernel, int parts, int threads, size_t smem) {
-  struct Known { const void* kernel; int parts, clusters; };
+  struct Known { const void* kernel; int parts; size_t smem; int clusters; };
   static thread_local Known known[128];
   static thread_local int n_known = 0;
   for (int i = 0; i < n_known; ++i)
-    if (known[i].kernel == (const void*)kernel && known[i].parts == parts) return known[i].clusters;
+    if (known[i].kernel == (const void*)kernel && known[i].parts == parts && known[i].smem == smem) return known[i].clusters;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(parts * 148));
   cfg.blockDim = dim3((unsigned)threads);
@@ -87,7 +87,7 @@ static int clusters_at_a_time(K kernel, int parts, int threads, size_t smem) {
     cudaGetLastError();
     n = 0;
   }
-  if (n_known < 128) known[n_known++] = {(const void*)kernel, parts, n};
+  if (n_known < 128) known[n_known++] = {(const void*)kernel, parts, smem, n};
   return n;
 }
 

@@ -196,7 +196,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     // and looked at only when it is needed, which is after its trip
     auto page_of = [&](int j) {
       const int key = (t_lo + j) * KEYS + lane * 16;
-      return (lane >= GROUPS || j >= n || key >= hi || key + 15 < lo) ? -1 : bt[key >> p.page_shift] & 0x7fffffff;
+      return (lane >= GROUPS || j >= n || key >= hi || key + 15 < lo) ? -1 : page_id(bt + (key >> p.page_shift));
     };
     auto checked = [&](int page) {
       if (page < p.n_pages) return page;
@@ -671,7 +671,11 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   pdl_trigger();
   tc_fence_before();
   __syncthreads();
-  if (warp == 11) tmem_dealloc(tmem_slot, 512);
+  if (warp == 11) {
+    if (abort_flag)
+      for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // products still on their way end before their memory is given back
+    tmem_dealloc(tmem_slot, 512);
+  }
   if (p.second) pdl_wait();
 }
 

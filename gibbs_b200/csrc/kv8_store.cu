@@ -264,7 +264,7 @@ __global__ void __launch_bounds__(128) kv8_store_rows_kernel(const Store p) {
   constexpr int TPR = HD / 8, SLOTS = 128 / TPR;
   __shared__ __align__(16) float2 cs[HD / 2];
   pdl_trigger();
-  const int r = blockIdx.y, sub = threadIdx.x % TPR, slot = (int)blockIdx.x * SLOTS + threadIdx.x / TPR;
+  const int r = blockIdx.x, sub = threadIdx.x % TPR, slot = (int)blockIdx.y * SLOTS + threadIdx.x / TPR;
   const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
   const bool active = slot < slots;
   const bool is_q = slot < p.heads, is_k = !is_q && slot < p.heads + p.kv_heads;
@@ -448,7 +448,7 @@ int launch_fast(const Store& p, long long segments, cudaStream_t stream) {
   const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
   if (p.step.one_each) {
     constexpr int SLOTS = 128 / (HD / 8);
-    gb_launch(kv8_store_rows_kernel<T, HD>, dim3((slots + SLOTS - 1) / SLOTS, p.step.n_requests), dim3(128), 0, stream, p);
+    gb_launch(kv8_store_rows_kernel<T, HD>, dim3(p.step.n_requests, (slots + SLOTS - 1) / SLOTS), dim3(128), 0, stream, p);
     return GB_OK;
   }
   // heads of a block: whole rounds of its warps, as many as leave four blocks for every SM

@@ -121,15 +121,16 @@ def _is(ok: bool, message: str) -> None:
 # The checks of a call are made twice over: as one expression, which is what a good call costs (a decode step makes a dozen of
 # them), and one by one with their messages where that expression is false.
 
-def _step_ok(step, block_table, rows: int, index: int) -> bool:
+def _step_ok(step, block_table, page_size: int, rows: int, index: int) -> bool:
     n, a, b, c = step.n_requests, step.q_start, step.q_len, step.start_pos
     return (a.dtype is _I32 and b.dtype is _I32 and c.dtype is _I32 and a.get_device() == index and b.get_device() == index
             and c.get_device() == index and a.is_contiguous() and b.is_contiguous() and c.is_contiguous() and a.numel() >= n
             and b.numel() >= n and c.numel() >= n and block_table.dtype is _I32 and block_table.get_device() == index
-            and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[0] >= n and rows >= step.n_tokens)
+            and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[0] >= n and rows >= step.n_tokens
+            and block_table.shape[1] * page_size >= step.max_ctx_len)
 
 
-def _refuse_step(step, block_table, rows: int, index: int, what: str) -> None:
+def _refuse_step(step, block_table, page_size: int, rows: int, index: int, what: str) -> None:
     n = step.n_requests
     for t in (step.q_start, step.q_len, step.start_pos):
         _is(t.dtype is _I32 and t.get_device() == index and t.is_contiguous() and t.numel() >= n,
@@ -137,6 +138,8 @@ def _refuse_step(step, block_table, rows: int, index: int, what: str) -> None:
     _is(block_table.dtype is _I32 and block_table.get_device() == index and block_table.dim() == 2 and block_table.is_contiguous()
         and block_table.shape[0] >= n, f"{what}: the block table is contiguous int32 [{n} requests, entries] on cuda:{index}")
     _is(rows >= step.n_tokens, f"{what}: {rows} rows, the step has {step.n_tokens} tokens")
+    _is(block_table.shape[1] * page_size >= step.max_ctx_len,
+        f"{what}: block tables of {block_table.shape[1]} pages of {page_size} do not hold contexts of {step.max_ctx_len}")
 
 
 def _vector_ok(t, n: int, index: int) -> bool:
@@ -170,7 +173,7 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
             and _vector_ok(k_gain, head_dim, index) and (inv_freq is None or (
                 not rotary_dim % 2 and 0 <= rotary_dim <= head_dim and _vector_ok(inv_freq, rotary_dim // 2 + 1, index)))
             and (pages is None or (pages.kv_heads == kv_heads and pages.head_dim == head_dim and pages.index == index))
-            and _step_ok(step, block_table, rows, index)):
+            and _step_ok(step, block_table, 1 << 40 if pages is None else pages.page_size, rows, index)):
         _refuse_store(x, part, good, rows, cols, q_out, heads, kv_heads, head_dim, q_gain, k_gain, inv_freq, rotary_dim, step,
                       block_table, pages, index, dtype)
     if pages is not None:
@@ -203,7 +206,7 @@ def _refuse_store(x, part, good, rows, cols, q_out, heads, kv_heads, head_dim, q
     _f32vec(inv_freq, rotary_dim // 2 + 1, "rotary table")
     _is(pages is None or (pages.kv_heads, pages.head_dim, pages.index) == (kv_heads, head_dim, index),
         "kv8 store: the pages hold another number of kv heads, other heads, or lie on another device")
-    _refuse_step(step, block_table, rows, index, "kv8 store")
+    _refuse_step(step, block_table, 1 << 40 if pages is None else pages.page_size, rows, index, "kv8 store")
     raise KernelError(f"kv8 store: all tensors lie on cuda:{index}")
 
 
@@ -216,7 +219,7 @@ def paged_attention(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, p
             and q.shape[1] == cols and out.shape[1] == cols and (qs[1] == 1 or cols == 1) and (os_[1] == 1 or cols == 1)
             and out.dtype is dtype and (dtype is _BF16 or dtype is _F32) and out.shape[0] >= step.n_tokens and out.get_device() == index
             and pages.kv_heads == kv_heads and pages.head_dim == head_dim and pages.index == index and window is not None and window >= 0
-            and _step_ok(step, block_table, q.shape[0], index)):
+            and (os_[0] >= cols or out.shape[0] == 1) and _step_ok(step, block_table, pages.page_size, q.shape[0], index)):
         _refuse_attention(q, heads, kv_heads, head_dim, pages, block_table, window, out, step, index)
     k, v, ks, vs = pages.addresses
     _call(1, index, q.device, (q.data_ptr(), qs[0], BF16 if dtype is _BF16 else F32, out.data_ptr(), os_[0], k, v, ks, vs, pages.n_pages,
@@ -235,5 +238,6 @@ def _refuse_attention(q, heads, kv_heads, head_dim, pages, block_table, window, 
     _is((pages.kv_heads, pages.head_dim, pages.index) == (kv_heads, head_dim, index) and out.get_device() == index,
         f"kv8 attention: the pages hold {pages.kv_heads} kv heads of {pages.head_dim} on {pages.device}")
     _is(window is not None and window >= 0, f"kv8 attention: a window of {window} keys (0: none)")
-    _refuse_step(step, block_table, q.shape[0], index, "kv8 attention")
+    _is(out.stride(0) >= out.shape[1] or out.shape[0] == 1, "kv8 attention: rows of out lie over one another")
+    _refuse_step(step, block_table, pages.page_size, q.shape[0], index, "kv8 attention")
     raise KernelError("kv8 attention: a call of these tensors is not taken")

@@ -546,6 +546,106 @@ def test_refusals():
             attend(**bad)
 
 
+def test_tables_that_do_not_hold_the_contexts_and_rows_over_one_another_are_refused():
+    from gibbs_b200.ops import KernelError, kv8
+    pages = make_pages(4, 2, 16, 64, torch.Generator().manual_seed(0))
+    q = torch.zeros(3, 4 * 64, dtype=torch.bfloat16, device=DEV)
+    x = torch.zeros(3, 8 * 64, dtype=torch.bfloat16, device=DEV)
+    bt = torch.zeros(1, 2, dtype=torch.int32, device=DEV)
+    for portions, behind in (([3], [30]), ([1], [32])):
+        with pytest.raises(KernelError, match="do not hold"):
+            kv8.qk_norm_rope_store(x, q, 4, 2, 64, None, None, EPS, None, 0, False, step_of(portions, behind), bt, pages)
+        with pytest.raises(KernelError, match="do not hold"):
+            kv8.paged_attention(q, 4, 2, 64, pages, bt, 0.125, 0, torch.empty_like(q), step_of(portions, behind))
+    with pytest.raises(KernelError, match="over one another"):
+        kv8.paged_attention(q, 4, 2, 64, pages, bt, 0.125, 0, q[:1].clone().expand(3, -1), step_of([3], [29]))
+    kv8.paged_attention(q[:1].expand(3, -1), 4, 2, 64, pages, bt, 0.125, 0, torch.empty_like(q), step_of([3], [29]))
+    # (rows of q alone need no pages, so no table that holds them)
+    kv8.qk_norm_rope_store(x, q, 4, 2, 64, None, None, EPS, None, 0, False, step_of([3], [300]), bt, None)
+
+
+WAYS = [(torch.bfloat16, [1, 1], 64, 16), (torch.bfloat16, [40, 2], 64, 16), (torch.bfloat16, [40], 128, 64), (torch.float32, [1, 3], 64, 16),
+        (torch.float32, [5], 48, 5)]
+
+
+@pytest.mark.parametrize("dt,portions,hd,page", WAYS)
+def test_windows_that_no_context_reaches(dt, portions, hd, page):
+    from gibbs_b200.ops import kv8
+    gen = torch.Generator().manual_seed(3)
+    behind = [100] * len(portions)
+    n_pages, bt = tables(portions, behind, page, random.Random(1))
+    pages = make_pages(n_pages, 2, page, hd, gen)
+    q = torch.randn(sum(portions), 4 * hd, generator=gen).to(dt).to(DEV)
+    outs = [kv8.paged_attention(q, 4, 2, hd, pages, bt.to(DEV), hd ** -0.5, w, torch.empty_like(q), step_of(portions, behind))
+            for w in (0, 2 ** 31 - 1, 2 ** 31 - 100, 2 ** 30, 2 ** 32 + 5, 2 ** 62)]
+    for o in outs[1:]:
+        assert torch.equal(o, outs[0])
+
+
+@pytest.mark.parametrize("dt,portions,hd,page", WAYS)
+@pytest.mark.parametrize("bad", [-2 ** 31, -2 ** 31 + 2, -7, 2 ** 31 - 1])
+def test_page_ids_far_outside(dt, portions, hd, page, bad):
+    from gibbs_b200.ops import kv8
+    gen = torch.Generator().manual_seed(3)
+    behind = [100] * len(portions)
+    n_pages, bt = tables(portions, behind, page, random.Random(1))
+    pages = make_pages(n_pages, 2, page, hd, gen)
+    q = torch.randn(sum(portions), 4 * hd, generator=gen).to(dt).to(DEV)
+    bt[0, 2] = bad
+    step = step_of(portions, behind)
+    kv8.paged_attention(q, 4, 2, hd, pages, bt.to(DEV), hd ** -0.5, 0, torch.empty_like(q), step)
+    assert int(step.status.item()) == 2
+    step.status.zero_()
+    before = [bits(t).clone() for t in pages.tensors()]
+    bt[:, 100 // page:] = bad
+    x = torch.randn(sum(portions), 8 * hd, generator=gen).to(dt).to(DEV)
+    kv8.qk_norm_rope_store(x, q, 4, 2, hd, None, None, EPS, None, 0, False, step, bt.to(DEV), pages)
+    assert int(step.status.item()) == 1
+    step.status.zero_()
+    assert all(torch.equal(bits(a), b) for a, b in zip(pages.tensors(), before))
+
+
+@pytest.mark.parametrize("dt", [torch.bfloat16, torch.float32])
+def test_more_requests_than_a_grid_has_rows(dt):
+    """70,001 requests of one token each: a token that sees itself alone gets its own value."""
+    from gibbs_b200.ops import kv8
+    n, hd = 70001, 64
+    gen = torch.Generator().manual_seed(9)
+    x = torch.randn(n, 4 * hd, generator=gen).to(dt).to(DEV)
+    pages = make_pages(n, 1, 16, hd, gen)
+    bt = torch.randperm(n, generator=gen).to(torch.int32).view(n, 1).to(DEV)
+    q, step = torch.empty(n, 2 * hd, dtype=dt, device=DEV), step_of([1] * n, [0] * n)
+    kv8.qk_norm_rope_store(x, q, 2, 1, hd, None, None, EPS, None, 0, False, step, bt, pages)
+    assert torch.equal(q, x[:, :2 * hd])
+    out = kv8.paged_attention(q, 2, 1, hd, pages, bt, 0.125, 0, torch.empty_like(q), step)
+    held = pages.dequantized()[1][bt[:, 0].long(), 0, 0]
+    half, smallest = 2.0 ** -4, 2.0 ** -10 * pages.v_scales[bt[:, 0].long()]
+    assert bool(((held - x[:, 3 * hd:].float()).abs() <= torch.maximum(half * x[:, 3 * hd:].float().abs(), smallest)).all())
+    # one weight over itself: 2^-11 for it in 16 bits, 2^-22 for it and for the quotient, and the output's own rounding
+    tol = (2.0 ** -11 + 2.0 ** -9 if dt == torch.bfloat16 else 0.0) + 2.0 ** -20
+    assert bool(((out.float().view(n, 2, hd) - held[:, None]).abs() <= tol * held[:, None].abs()).all())
+
+
+def test_calls_on_two_streams_at_once():
+    from gibbs_b200.ops import kv8
+    gen = torch.Generator().manual_seed(4)
+    calls = []
+    for portions, behind, hd, page in (([1] * 4, [9000, 8000, 100, 5], 128, 64), ([300, 1, 1], [4000, 3000, 17], 64, 16)):
+        n_pages, bt = tables(portions, behind, page, random.Random(1))
+        q = torch.randn(sum(portions), 8 * hd, generator=gen).to(torch.bfloat16).to(DEV)
+        calls.append((q, 8, 2, hd, make_pages(n_pages, 2, page, hd, gen), bt.to(DEV), hd ** -0.5, 0, torch.empty_like(q), step_of(portions, behind)))
+    want = [kv8.paged_attention(*c).clone() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, c in zip(streams, calls):
+            with torch.cuda.stream(s):
+                kv8.paged_attention(*c)
+    torch.cuda.synchronize()
+    for c, w in zip(calls, want):
+        assert torch.equal(c[8], w) and int(c[9].status.item()) == 0
+
+
 # ---------------------------------------------------------------------------------------------------
 def copy_groups(rows, gen):
     whole = torch.randint(0, 256, (rows + 2, 4096 * 5 + 64), dtype=torch.uint8, generator=gen).to(DEV)
