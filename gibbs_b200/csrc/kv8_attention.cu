@@ -16,7 +16,10 @@ namespace {
 
 using namespace kv8;
 
-constexpr int FEW = 32;              // rows of a request up to which it is not worth 256-row tiles
+// Rows of a request (its tokens times the heads of a kv head's group) up to which 256-row tiles are not worth their time, which does not
+// depend on the rows.  32 / 8 heads of 64, 4,000 keys, us by tiles of few rows / by 256 rows: at 48 rows 1 request 20 / 25, 8 48 / 52,
+// 32 135 / 159; at 64 rows 20 / 25, 55 / 52, 176 / 159; at 32 rows 18 / 25, 43 / 52, 92 / 159.
+constexpr int FEW = 48;
 constexpr int MAX_PARTS = 16;        // CTAs of a cluster that share a tile's keys, at most (8 is the portable limit)
 
 // A tile's request, rows and keys.
@@ -874,7 +877,7 @@ int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t st
   }
 }
 
-// Few tiles (a launch of few requests): one CTA of many warps for an SM, and a tile's keys shared by a cluster of them, as many as the
+// Few tiles (a launch of few requests, tiles of 8 rows): one CTA of many warps for an SM, and a tile's keys shared by a cluster of them, as many as the
 // chip holds at a time.  (Clusters of four-warp CTAs come to lie three or four on an SM and leave others empty: 4 requests of 32,000
 // keys, 32 / 8 heads of 128, 55 us.)  Many tiles: CTAs of four warps, several on an SM, so that one's beginning and end lie beside the
 // others' work.
@@ -895,18 +898,17 @@ int launch_mma_of(const Attn& p, long long tiles, long long keys, cudaStream_t s
     GB_FAIL(GB_ERR_CUDA, "kv8_attention: cuTensorMapEncodeTiled failed (%lld rows of %d)", rows, HD);
   const long long chunks = (keys + C::CK - 1) / C::CK, ctas = tiles * p.kv_heads;
   int parts = 1;
-  if (C::CTAS == 1) {
+  if (C::CTAS == 1)
     parts = parts_that_fit(kv8_attention_mma_kernel<HD, NB, WARPS>, 1, ctas, chunks, C::NW, SMEM);
-  } else {
+  else if (NB == 1)
     while (parts < MAX_PARTS && ctas * parts * 2 <= 148 * C::CTAS && chunks >= (long long)parts * 2 * C::NW) parts *= 2;
-  }
   return launch_parts(kv8_attention_mma_kernel<HD, NB, WARPS>, p, parts, tiles, 32 * C::NW, SMEM, stream, mk, mv);
 }
-template <int HD, int NB>
-int launch_mma(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
-  // (tiles of 16 rows need twice the registers: eight warps)
-  constexpr int MANY = NB == 2 ? 8 : HD == 64 ? 16 : 12;
-  return tiles * p.kv_heads <= 148 ? launch_mma_of<HD, NB, MANY>(p, tiles, keys, stream) : launch_mma_of<HD, NB, 4>(p, tiles, keys, stream);
+template <int HD>
+int launch_mma(const Attn& p, bool rows16, long long tiles, long long keys, cudaStream_t stream) {
+  if (rows16) return launch_mma_of<HD, 2, 4>(p, tiles, keys, stream);
+  return tiles * p.kv_heads <= 148 ? launch_mma_of<HD, 1, HD == 64 ? 16 : 12>(p, tiles, keys, stream)
+                                   : launch_mma_of<HD, 1, 4>(p, tiles, keys, stream);
 }
 
 }  // namespace
@@ -959,13 +961,18 @@ GB_OP(gb_op_kv8_attention) {
     p.few = FEW;
     p.first = 1;
   }
-  // rows of a tile: with 8, a step of single tokens in groups of eight heads or fewer, and what stands beside wide portions (single
-  // tokens as a rule); with 16, half as many passes over the keys
-  const bool small = wide || (long long)p.step.max_q * group <= 8;
   // upper bound of the tiles: sum_r ceil(q_len_r * group / rt)
-  const int rt = !mma ? 4 : small ? 8 : 16;
-  long long tiles = p.step.one_each ? (long long)p.step.n_requests * ((group + rt - 1) / rt)
-                                    : (long long)p.step.n_tokens * group / rt + p.step.n_requests;
+  auto tiles_of = [&](int rt) {
+    return p.step.one_each ? (long long)p.step.n_requests * ((group + rt - 1) / rt)
+                           : (long long)p.step.n_tokens * group / rt + p.step.n_requests;
+  };
+  int rt = mma ? 8 : 4;
+  long long tiles = tiles_of(rt);
+  // Tiles of 16 rows: half as many passes over the keys, once the tiles of 8 are more than the SMs hold at a time.  32 / 8 heads of 128,
+  // 4,000 keys, 12 rows a request, us with 8 / 16: 32 requests 98 / 70; 8 requests 37 / 41, 2 requests 22 / 26.  (What stands beside
+  // wide portions is single tokens as a rule, in groups of 8 heads at most.)
+  const bool rows16 = mma && !wide && (long long)p.step.max_q * group > 8 && tiles * p.kv_heads > 148 * (p.hd == 64 ? 4 : 3);
+  if (rows16) tiles = tiles_of(rt = 16);
   if (wide) {                                                  // (the requests that are left have FEW rows at most)
     const long long most = (long long)p.step.n_requests * ((FEW + rt - 1) / rt);
     tiles = tiles < most ? tiles : most;
@@ -974,8 +981,7 @@ GB_OP(gb_op_kv8_attention) {
   const long long keys = p.window > 0 && p.window + rt < p.step.max_ctx ? p.window + rt : p.step.max_ctx;
   int rc;
   if (mma)
-    rc = p.hd == 64 ? (small ? launch_mma<64, 1>(p, tiles, keys, ctx->stream) : launch_mma<64, 2>(p, tiles, keys, ctx->stream))
-                    : (small ? launch_mma<128, 1>(p, tiles, keys, ctx->stream) : launch_mma<128, 2>(p, tiles, keys, ctx->stream));
+    rc = p.hd == 64 ? launch_mma<64>(p, rows16, tiles, keys, ctx->stream) : launch_mma<128>(p, rows16, tiles, keys, ctx->stream);
   else
     rc = dtype == GB_F32 ? dispatch_any<float>(p, tiles, keys, ctx->stream) : dispatch_any<bf16>(p, tiles, keys, ctx->stream);
   if (rc != GB_OK) return rc;

@@ -688,10 +688,12 @@ int launch(const Attn& p, long long tiles, long long keys, cudaStream_t stream) 
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_tcgen05_kernel<HD>, cudaFuncAttributeMaxDynamicSharedMemorySize, Cfg<HD>::SMEM));
     attr_set = true;
   }
-  // CTAs that share a tile's keys: as many as the SMs hold at a time, each with four key tiles at least.  `tiles` is an upper bound
-  // that counts one for every request; the CTAs that have long walks are those of the longest portion, or of all tokens together.
-  const int two = 2 * (ROWS / (p.heads / p.kv_heads));
-  const long long longest = (p.step.max_q + two - 1) / two, all = p.step.n_tokens / two, walks = (longest > all ? longest : all) * p.kv_heads;
+  // CTAs that share a tile's keys: as many as the SMs hold at a time, each with four key tiles at least.  `tiles` is an upper bound that
+  // counts one for every request; how many there are is estimated from the longest portion and the mean of the others, which are
+  // taken to be as long as their mean, or, where that is few rows, to be single tokens and a portion that has the rest of them.
+  const long long two = 2 * (ROWS / (p.heads / p.kv_heads)), others = p.step.n_requests - 1, rest = p.step.n_tokens - p.step.max_q;
+  const bool alike = others > 0 && rest * (p.heads / p.kv_heads) > others * p.few;
+  const long long walks = ((p.step.max_q + two - 1) / two + (alike ? others * ((rest / others + two - 1) / two) : (rest + two - 1) / two)) * p.kv_heads;
   const long long most = (keys + KEYS - 1) / KEYS / 4;
   int parts = 1;
   for (int x = 2; x <= MAX_SHARES && x <= most; ++x)
