@@ -122,7 +122,8 @@ __device__ __forceinline__ void join(const Attn& p, const Tile& t, int kvh, int 
 }
 
 // ---------------------------------------------------------------- any type, head size and page size
-// A warp takes chunks of 32 keys: for the scores a lane has a key, for the output it has pairs of columns.
+// A warp takes chunks of 32 keys: for the scores a lane has a key, for the output it has pairs of columns.  Bound by the trips of a chunk
+// (page, scales, a key's bytes piece by piece): 9 requests of 2,000 keys, 24 / 8 heads of 48 in 32 bits, 45 us.
 template <typename T, int NP>
 __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
   constexpr int RT = 4, NW = 4;
@@ -256,7 +257,9 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
 // The 32-bit path (and bfloat16 heads that the kernels below do not take).  Tiles of 4 rows; a warp takes chunks of 32 keys.  HD / 8
 // lanes share a key, eight bytes each, of K and of V alike, so all loads of a chunk are whole lines and go out together.  A lane's
 // partial scores of its keys are added and handed out in one go (each step exchanges half of them), and end as the scores of ONE key
-// in every lane; weights go back through shared memory.  Bound by FMAs: 2 HD 4 of them for a key.
+// in every lane; weights go back through shared memory.  Bound by a chunk's chain (loads, conversions, sums
+// over lanes, softmax) with three warps a scheduler: 64 requests of 2,048 keys, 32 / 8 heads of 64, 97 us, 11 TFLOP/s; nine requests of 1 to
+// 4,002 keys, 24 / 8 heads, 14.1 us.
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
   constexpr int RT = 4, NW = 4, LPR = HD / 8, KG = 32 / LPR, KEYS = 32 / KG;       // lanes of a key, keys at a time, keys of a lane
@@ -435,6 +438,8 @@ __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
 // the warp's own, and a copy costs an instruction instead of one for every lane and piece.  The rows are swizzled (128-byte
 // rows by the 16-byte piece XOR row, 64-byte rows by piece XOR row / 2) and the keys of a group take the places pi(0..15) of the
 // products: with these every fragment is read without a bank conflict.
+// Bound by memory and by how evenly the CTAs lie on the SMs: 64 requests of 2,112 keys, 32 / 8 heads of 64, 30.3 us, 4.6 TB/s of the
+// cache's 139 MB; 4 requests of 30,000 to 32,768 keys, 32 / 8 heads of 128, 48.0 us, 5.4 TB/s; one request of 2,048 keys 7.3 us, by its trips.
 template <int HD, int WARPS> struct Mma {
   static constexpr int NW = WARPS;
   static constexpr int NG = 2;                                 // groups of a slot, taken together
@@ -830,7 +835,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
 }
 
 // ---------------------------------------------------------------- launches
-// How many CTAs share a tile's keys, a chunk for every warp at least: as many as let the chip hold `over` times what is launched.
+// How many CTAs share a tile's keys, a chunk for every warp at least: as many as make no more than `over` times what the chip holds.
 template <typename K>
 int parts_that_fit(K kernel, int over, long long ctas, long long chunks, int warps, size_t smem) {
   int parts = 1;
@@ -848,6 +853,8 @@ int launch_any(const Attn& p, long long tiles, long long keys, cudaStream_t stre
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_any_kernel<T, NP>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set = true;
   }
+  // (Once what the chip holds.  24 / 8 heads of 256, us with once / twice: nine requests of 2,000 keys 209 / 285, of 1 to 4,002 304 / 205; of 48:
+  // 45 / 53 and 71 / 46.)
   const int parts = parts_that_fit(kv8_attention_any_kernel<T, NP>, 1, tiles * p.kv_heads, (keys + 31) / 32, NW, smem);
   return launch_parts(kv8_attention_any_kernel<T, NP>, p, parts, tiles, 32 * NW, smem, stream);
 }
@@ -859,6 +866,8 @@ int launch_rows(const Attn& p, long long tiles, long long keys, cudaStream_t str
     GB_CUDA(cudaFuncSetAttribute(kv8_attention_rows_kernel<T, HD>, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
     attr_set = true;
   }
+  // (Twice what the chip holds: requests of a step differ in length, and the CTAs of short ones leave at once.  24 / 8 heads of 64, us with
+  // once / twice: nine requests of 1 to 4,002 keys 28 / 23, eight of 100 to 8,000 37 / 33; nine of 2,000 25 / 31.)
   const int parts = parts_that_fit(kv8_attention_rows_kernel<T, HD>, 2, tiles * p.kv_heads, (keys + 31) / 32, NW, SMEM);
   return launch_parts(kv8_attention_rows_kernel<T, HD>, p, parts, tiles, 32 * NW, SMEM, stream);
 }
@@ -877,10 +886,11 @@ int dispatch_any(const Attn& p, long long tiles, long long keys, cudaStream_t st
   }
 }
 
-// Few tiles (a launch of few requests, tiles of 8 rows): one CTA of many warps for an SM, and a tile's keys shared by a cluster of them, as many as the
-// chip holds at a time.  (Clusters of four-warp CTAs come to lie three or four on an SM and leave others empty: 4 requests of 32,000
-// keys, 32 / 8 heads of 128, 55 us.)  Many tiles: CTAs of four warps, several on an SM, so that one's beginning and end lie beside the
-// others' work.
+// Few tiles (a launch of few requests, tiles of 8 rows): one CTA of many warps for an SM, and a tile's keys shared by a cluster of
+// them, as many as the chip holds at a time.  (Clusters of four-warp CTAs come to lie three or four on an SM and leave others empty: 4 requests of 32,000
+// keys, 32 / 8 heads of 128, 55 us against 48.)  Many tiles: CTAs of four warps, several on an SM, so that one's beginning and end lie
+// beside the others' work.  2,000 keys, 32 / 8 heads of 64, us by many warps / by four: 16 requests 20 / 29, 24 requests 31 / 25, 64 requests
+// 57 / 43; with heads of 128 29 / 31, 41 / 36, 76 / 82.
 template <int HD, int NB, int WARPS>
 int launch_mma_of(const Attn& p, long long tiles, long long keys, cudaStream_t stream) {
   using C = Mma<HD, WARPS>;
@@ -947,7 +957,8 @@ GB_OP(gb_op_kv8_attention) {
   p.page_shift = 0;
   while ((1 << p.page_shift) < p.page_size) ++p.page_shift;
   const bool mma = dtype == GB_BF16 && (p.hd == 64 || p.hd == 128) && p.page_size >= 16 &&
-                   (1 << p.page_shift) == p.page_size && (long long)p.n_pages * p.kv_heads * p.page_size < 0x7fffffff && p.ldq % 8 == 0 && ((uintptr_t)p.q & 15) == 0;
+                   (1 << p.page_shift) == p.page_size && (long long)p.n_pages * p.kv_heads * p.page_size < 0x7fffffff &&
+                   p.ldq % 8 == 0 && ((uintptr_t)p.q & 15) == 0;
   // Requests of more than FEW rows go to tcgen05, which takes 256 rows at a time; they have to lie on 16-byte boundaries.
   const bool wide = mma && (long long)p.step.max_q * group > FEW && group <= 64 && p.ldo % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
   p.few = 0x7fffffff;

@@ -8,11 +8,16 @@
 //                into a ring of swizzled tiles; K_j brings the scales of its pages along
 //   warp 11      one thread issues S = Q K_j^T for both row tiles and, when a tile's weights are there, O += P V_j and the next S
 //   warps 0-7    a thread has a row: reads S from tensor memory, scales, masks, running maximum and sum in 32 bits, writes the
-//                weights in f16 over S in tensor memory, from where they are the A operand of the second product
+//                weights in f16 to tensor memory, from where they are the A operand of the second product
 //
-// The two row tiles take turns: while one is in its softmax the other's products run, and both use the same converted K and V,
-// which halves the conversion's share (it costs about a fifth of the instructions).  Bound by the special-function unit: a 2^x
-// for every (row, key) at 16 a cycle, 1,024 cycles a tile against some 512 (head_dim 64) of the tensor cores.
+// The two row tiles take turns: while one is in its softmax the other's products run, and both use the same converted K and V.  (Products
+// issued as either tile is ready, without that order: 48 us against 47 at 2,048 tokens, 345 against 326 at 8,192.)
+//
+// 2,048 tokens, 32 / 8 heads of 64: 47 us, 366 TFLOP/s; 8,192 tokens, 16 / 4 heads of 128: 326 us, 843 TFLOP/s.  What bounds it, from copies
+// that leave work out: heads of 64 take 45 us without the 2^x, 40 without any softmax, 34 without conversion and loads either, so it is
+// the hand-overs of a key tile (scores to registers, weights back, product) and a CTA's beginning and end; heads of 128 take 301 us
+// without conversion, 296 without softmax and 229 without both.  The special-function unit is at 37 % (a share of the 2^x by a
+// polynomial is slower: 49 and 341 us).
 //
 // Scales, as in the kernel for few rows: q's row under the power of two that brings its largest magnitude to 2^14; a score
 // times the inverse and the scale of K's page; the scale of V's page in the exponent, x_j = score_j + log2(scale_j), weights
@@ -281,8 +286,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
         for (int y = 0; y < MINE; ++y)
 #pragma unroll
           for (int i = 0; i < PER; ++i)
-            w[y][i] = *reinterpret_cast<const uint4*>(mine + (size_t)(it % C::STAGES) * C::RAW_TILE + min(w0 + y * (CONVERTERS / 32), GROUPS - 1) * 16 * HD +
-                                                      i * 512);
+            w[y][i] = *reinterpret_cast<const uint4*>(mine + (size_t)(it % C::STAGES) * C::RAW_TILE +
+                                                      min(w0 + y * (CONVERTERS / 32), GROUPS - 1) * 16 * HD + i * 512);
         if (!__all_sync(0xffffffffu, mbar_wait(&kv_empty[s], ((it / C::RING) & 1) ^ 1) && !abort_flag)) {
           abort_flag = 1;
           if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT);
@@ -690,10 +695,12 @@ int launch(const Attn& p, long long tiles, long long keys, cudaStream_t stream) 
   }
   // CTAs that share a tile's keys: as many as the SMs hold at a time, each with four key tiles at least.  `tiles` is an upper bound that
   // counts one for every request; how many there are is estimated from the longest portion and the mean of the others, which are
-  // taken to be as long as their mean, or, where that is few rows, to be single tokens and a portion that has the rest of them.
+  // taken to be as long as their mean, or, where that is few rows, to be single tokens and a portion that has the rest of them.  (Without
+  // the others 8 requests of 16 tokens behind 4,000 keys, 32 / 8 heads of 64, take 79 us, by eight CTAs a tile; with them 52, by two.)
   const long long two = 2 * (ROWS / (p.heads / p.kv_heads)), others = p.step.n_requests - 1, rest = p.step.n_tokens - p.step.max_q;
   const bool alike = others > 0 && rest * (p.heads / p.kv_heads) > others * p.few;
-  const long long walks = ((p.step.max_q + two - 1) / two + (alike ? others * ((rest / others + two - 1) / two) : (rest + two - 1) / two)) * p.kv_heads;
+  const long long of_others = alike ? others * ((rest / others + two - 1) / two) : (rest + two - 1) / two;
+  const long long walks = ((p.step.max_q + two - 1) / two + of_others) * p.kv_heads;
   const long long most = (keys + KEYS - 1) / KEYS / 4;
   int parts = 1;
   for (int x = 2; x <= MAX_SHARES && x <= most; ++x)

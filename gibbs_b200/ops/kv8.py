@@ -6,7 +6,7 @@ page's scale is the smallest 2^e, -64 <= e <= 50, that holds its rows' largest m
 page gets its first row and only grows from there; when it grows, the rows that the page holds are rounded again.  A
 magnitude is off by at most half a step of e4m3, 2^-4 of it, and by 2^-10 of the scale below 2^-6 scales (a growing scale may
 add as much again there).  What is not finite, or above 448 * 2^50, is stored as NaN and makes the scale negative; it stays
-with the rows that see it.
+with the rows that see it.  Scales are the store's to write: the attention takes them to be such powers of two.
 
 Both operations take the engine's ``StepState``: which requests a step has, where each begins, how much it brings and how
 much it holds already.  As everywhere in this package a step's metadata (its int32 tensors and the block table) lies in place
@@ -153,7 +153,7 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
     ``q_out`` [tokens, heads * head_dim], k and v into their pages.  ``qkv``: rows [q heads | k heads | v heads], or the
     ``ops.Partials`` of their product.  ``inv_freq``: rotary_dim / 2 frequencies, or those and the factor on cosines and sines
     behind them.  ``pages`` None: rows of q alone (a layer that reads another layer's cache).  Only rows of the step's tokens
-    are read or written."""
+    are read or written.  A step writes to pages that no other request of it holds."""
     part = None if isinstance(qkv, torch.Tensor) else qkv
     x = qkv if part is None else part.ws
     index, cols = x.get_device(), (heads + (2 * kv_heads if pages is not None else 0)) * head_dim
@@ -213,7 +213,8 @@ def _refuse_store(x, part, good, rows, cols, q_out, heads, kv_heads, head_dim, q
 def paged_attention(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, pages: Pages, block_table: torch.Tensor,
                     scale: float, window: int, out: torch.Tensor, step) -> torch.Tensor:
     """out[t, h, :] = softmax over visible keys of (q.K)*scale, times V, over an 8-bit cache; q may be a column slice of a
-    wider row.  Rows of ``out`` behind the step's tokens are left as they are."""
+    wider row.  ``window`` 0: none; block tables hold the step's longest context.  Rows of ``out`` behind the step's tokens are left as
+    they are."""
     index, cols, qs, os_, dtype = q.get_device(), heads * head_dim, q.stride(), out.stride(), q.dtype
     if not (index >= 0 and heads > 0 and kv_heads > 0 and not heads % kv_heads and len(qs) == 2 and len(os_) == 2
             and q.shape[1] == cols and out.shape[1] == cols and (qs[1] == 1 or cols == 1) and (os_[1] == 1 or cols == 1)
