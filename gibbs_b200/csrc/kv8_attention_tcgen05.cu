@@ -195,7 +195,10 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     constexpr int PIECES = HD / 16, PER = 16 * PIECES / 32;   // 16-byte pieces of a row; of a group, for a lane
     constexpr int ROWS_STEP = 32 / PIECES;                    // rows from one of a lane's pieces to the next
     constexpr int MINE = (GROUPS + CONVERTERS / 32 - 1) / (CONVERTERS / 32);
-    const int w0 = warp - 8, piece = lane % PIECES, row_in = lane / PIECES;      // groups w0, w0 + 3, w0 + 6 < 8
+    // (The f16 of pieces 4..7 go to the banks of those of pieces 0..3, a sub-tile further: eight lanes that store together have the lower
+    // pieces of one row and the upper ones of its neighbour, which the swizzle puts elsewhere.)
+    const int w0 = warp - 8, piece = lane % PIECES, row_in = (lane / PIECES) ^ (piece >> 2);     // groups w0, w0 + 3, w0 + 6 < 8
+    const int spot = (row_in * PIECES + piece) * 16;          // of this lane among the 512 bytes of a warp's copy
     const int* bt = p.block_table + (size_t)r * p.bt_stride;
     // lane i < 8: page of group i of a tile, -1 where nothing of it is visible (and in the other lanes); as it comes from the table,
     // and looked at only when it is needed, which is after its trip
@@ -208,7 +211,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
       if (warp == 8) atomicExch(p.status, STATUS_BAD_PAGE_READ);
       return -1;
     };
-    uint8_t* mine = sraw + lane * 16;
+    uint8_t* mine = sraw + spot;
     const uint32_t mine_at = smem_u32(mine) + w0 * 16 * HD;
     const size_t head = (size_t)kvh << p.page_shift;
     size_t at[MINE];                                          // where this warp's groups of the last tile asked for lie in the pool
@@ -226,7 +229,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
             rows[y] = pg < 0 || g >= GROUPS ? 0 : hi - key - row_in;
           }
         }
-        const uint8_t* pool = ((it & 1) ? p.v_pages : p.k_pages) + lane * 16;
+        const uint8_t* pool = ((it & 1) ? p.v_pages : p.k_pages) + spot;
         const uint32_t dst = mine_at + (uint32_t)((it % C::STAGES) * C::RAW_TILE);
 #pragma unroll
         for (int y = 0; y < MINE; ++y) {
