@@ -257,9 +257,9 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
 // The 32-bit path (and bfloat16 heads that the kernels below do not take).  Tiles of 4 rows; a warp takes chunks of 32 keys.  HD / 8
 // lanes share a key, eight bytes each, of K and of V alike, so all loads of a chunk are whole lines and go out together.  A lane's
 // partial scores of its keys are added and handed out in one go (each step exchanges half of them), and end as the scores of ONE key
-// in every lane; weights go back through shared memory.  Bound by a chunk's chain (loads, conversions, sums
-// over lanes, softmax) with three warps a scheduler: 64 requests of 2,048 keys, 32 / 8 heads of 64, 97 us, 11 TFLOP/s; nine requests of 1 to
-// 4,002 keys, 24 / 8 heads, 14.1 us.
+// in every lane; weights go back through shared memory.  Bound by a chunk's chain (loads, conversions, sums over lanes, softmax) with
+// three warps a scheduler: 64 requests of 2,048 keys, 32 / 8 heads of 64, 97 us, 11 TFLOP/s; nine requests of 1 to 4,002 keys, 24 / 8 heads,
+// 14.1 us; a prompt of 2,048 tokens 893 us, 19 TFLOP/s (with pairs of FMAs, whose operands have to be moved together, 1,020).
 template <typename T, int HD>
 __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
   constexpr int RT = 4, NW = 4, LPR = HD / 8, KG = 32 / LPR, KEYS = 32 / KG;       // lanes of a key, keys at a time, keys of a lane
