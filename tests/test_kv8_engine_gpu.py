@@ -276,3 +276,81 @@ def test_several_answers_to_a_prompt(tmp_path_factory, dtype, cache_dtype):
         each = [SamplingParams(temperature=1.0, top_k=50, max_new_tokens=12, seed=9 + i) for i in range(6)]
         assert got == make().generate([prompt] * 6, each, stop_at_eos=False)
     assert gen.engine.cache.free_pages() == [64]
+
+
+# Each of two engines is within 2e-4 of its formulas in float32 (the bound of those designs' own tests).
+@pytest.mark.parametrize("n", [13, 16, 61])
+@pytest.mark.parametrize("name", ["A", "B", "C"])
+@pytest.mark.parametrize("design", ["potivik", "petelix", "sisadra", "selivik", "guvetar", "nutopel"])
+def test_forks_in_every_design(design, name, n):
+    """State slots, latent rows, windows that keep a sequence's beginning, blocks of positions, tokens before: all go with a fork."""
+    import importlib
+    from gibbs_b200 import Engine, StepEntry
+    h = importlib.import_module(design + "_helpers")
+    cfg, seed = h.CONFIGS[name]
+    key = (design, name)
+    if key not in _models:
+        _models[key] = h.build(name, "float32")[2] if design == "potivik" else h.build(cfg, seed, "float32")[1]
+    make = lambda: Engine(_models[key], n_pages=96, page_size=16, max_requests=4, max_step_tokens=512, max_context=512, guard_cache=True)  # noqa: E731
+    vocab = cfg["vocab"] if "vocab" in cfg else _models[key].vocab_size
+    ids, tails = random_ids(1, n, vocab), [random_ids(2 + i, 24, vocab) for i in range(2)]
+    tails[1][0] = tails[0][0]
+    eng = make()
+    eng.open("p")
+    eng.step([StepEntry("p", ids, [n - 1])])
+    eng.fork("p", "c")
+    got = [[], []]
+    for t in range(16):                                          # single tokens, beside each other
+        rows = eng.step([StepEntry("p", [tails[0][t]], [0]), StepEntry("c", [tails[1][t]], [0])])
+        assert t or torch.equal(rows[0], rows[1])
+        for i in range(2):
+            got[i].append(rows[i].cpu().numpy().copy())
+    eng.close("p")
+    got[1] += list(eng.step([StepEntry("c", tails[1][16:], list(range(8)))]).cpu().numpy())
+    eng.check_status(), eng.cache.check()
+    alone = make()
+    for i, tail in enumerate(tails):
+        tail = tail if i else tail[:16]
+        steps = [{"entries": [{"id": "r", "tokens": ids, "want": []}], "end": []}]
+        steps += [{"entries": [{"id": "r", "tokens": [t], "want": [0]}], "end": []} for t in tail[:16]]
+        if i:
+            steps += [{"entries": [{"id": "r", "tokens": tail[16:], "want": list(range(8))}], "end": []}]
+        steps[-1]["end"] = ["r"]
+        bad = first_wrong(np.stack(got[i]), run_trace_on_engine(alone, steps)["r"], 4e-4)
+        assert bad is None, (i, bad)
+    eng.close("c")
+    assert eng.cache.free_pages() == [96] * len(eng.cache.groups)
+
+
+@pytest.mark.parametrize("cache_dtype", [None, "float8_e4m3"])
+@pytest.mark.parametrize("n", [20, 33, 80])
+def test_forks_with_windows_and_shared_caches(n, cache_dtype):
+    """A window gives shared pages back, one holder after the other, while both requests go on."""
+    from gibbs_b200 import StepEntry
+    from gibbs_b200.parts import build_model
+    from gibbs_b200.weights import TensorDict, expected_tensors
+    plan = _attention_plan(64, 24)
+    torch.manual_seed(3)
+    tensors = {}
+    for name, decl in expected_tensors(plan).items():
+        shape = decl.shapes[0]
+        tensors[name] = 1 + 0.1 * torch.randn(shape) if len(shape) == 1 else torch.randn(shape) * (0.3 if name == "emb" else 1 / math.sqrt(shape[-1]))
+    model = build_model(plan, TensorDict(tensors), torch.float32, DEV)
+    ids, tails = random_ids(1, n, 300), [random_ids(2 + i, 40, 300) for i in range(2)]
+    eng, alone = (_engine(model, n_pages={None: 40, 24: 40}, cache_dtype=cache_dtype) for _ in range(2))
+    eng.open("p")
+    eng.step([StepEntry("p", ids, [n - 1])])
+    eng.fork("p", "c")
+    got = [[], []]
+    for t in range(40):
+        rows = eng.step([StepEntry("p", [tails[0][t]], [0]), StepEntry("c", [tails[1][t]], [0])]).cpu().numpy()
+        eng.check_status(), eng.cache.check()
+        for i in range(2):
+            got[i].append(rows[i].copy())
+    eng.close("p"), eng.close("c")
+    assert eng.cache.free_pages() == [40, 40]
+    for i, tail in enumerate(tails):
+        steps = [{"entries": [{"id": "r", "tokens": ids, "want": []}], "end": []}]
+        steps += [{"entries": [{"id": "r", "tokens": [t], "want": [0]}], "end": []} for t in tail]
+        steps[-1]["end"] = ["r"]
+        assert first_wrong(np.stack(got[i]), run_trace_on_engine(alone, steps)["r"], 2 * TOL8["float32"]) is None
