@@ -36,6 +36,7 @@ using namespace sm100;
 constexpr int ROWS = 128, KEYS = 128, GROUPS = KEYS / 16;
 constexpr int THREADS = 384;                                  // 8 softmax warps, 3 that convert, 1 that issues: 168 registers a thread
 constexpr int CONVERTERS = 96;
+constexpr int AFTER = 0;
 constexpr int META = 4;                                       // tiles whose scales are kept
 
 template <int HD> struct Cfg {
@@ -105,6 +106,12 @@ __device__ __forceinline__ float4 ld_cluster_f4(const float4* p, int rank) {
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(cluster_addr(p, rank)) : "memory");
   return v;
+}
+
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float r;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
+  return r;
 }
 
 template <int HD>
@@ -518,12 +525,12 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
 #pragma unroll
       for (int g = 0; g < GROUPS; ++g) {
         const float* u = v + 16 * g;
-        float a = fmaxf(fmaxf(u[0], u[1]), u[2]), b = fmaxf(fmaxf(u[3], u[4]), u[5]);
-        a = fmaxf(fmaxf(a, u[6]), u[7]);
-        b = fmaxf(fmaxf(b, u[8]), u[9]);
-        a = fmaxf(fmaxf(a, u[10]), u[11]);
-        b = fmaxf(fmaxf(b, u[12]), u[13]);
-        a = fmaxf(fmaxf(a, u[14]), u[15]);
+        float a = max3(u[0], u[1], u[2]), b = max3(u[3], u[4], u[5]);
+        a = max3(a, u[6], u[7]);
+        b = max3(b, u[8], u[9]);
+        a = max3(a, u[10], u[11]);
+        b = max3(b, u[12], u[13]);
+        a = max3(a, u[14], u[15]);
         const float2 sc = *reinterpret_cast<const float2*>(&mt[g]);
         // (a factor that underflowed would make NaN of a masked column's -inf)
         top = fmaxf(top, fmaf(fmaxf(a, b), fmaxf(factor * sc.x, 1.2e-38f), sc.y));
@@ -575,13 +582,20 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
           float a, b;
           upk2(add2(sum[0], sum[1]), a, b);
           l = fmaf(a + b, sc.z, l);
+          if (half == 1 && g == AFTER) {                       // (the first half's weights have arrived meanwhile)
+            tmem_st_wait();
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&p_full[x][0]);
+          }
         }
         tmem_st_16_issue(tmem_px + lane_off + (uint32_t)(32 * half), packed);
         tmem_st_16_issue(tmem_px + lane_off + (uint32_t)(32 * half + 16), packed + 16);
-        tmem_st_wait();
-        tc_fence_before();
-        __syncwarp();
-        if (half == 0 && lane == 0) mbar_arrive(&p_full[x][0]);
+        if (half == 1) {
+          tmem_st_wait();
+          tc_fence_before();
+          __syncwarp();
+        }
       }
       if (marks[j % META]) {
         // values of the tile's pages that are NaN, for the keys that the row sees
