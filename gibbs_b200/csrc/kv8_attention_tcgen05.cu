@@ -493,7 +493,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     const uint32_t tmem_x = x ? tmem_s[1] : tmem_s[0], tmem_ox = x ? tmem_o[1] : tmem_o[0], tmem_px = x ? tmem_p[1] : tmem_p[0];
     const int n_mine = x ? n_x[1] : n_x[0];
     for (int j = 0; j < n_mine; ++j) {
-      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1) && !abort_flag)) {
+      if (!__all_sync(0xffffffffu, mbar_wait(&s_full[x], j & 1))) {
         abort_flag = 1;
         if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT + 2);
         alive = false;
@@ -502,6 +502,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
       tc_fence_after();
       const int col0 = (t_lo + j) * KEYS;
       const float4* mt = meta[j % META];
+      const bool marked = marks[j % META] != 0;
       const bool full = col0 + KEYS - 1 <= pos_first && (p.window <= 0 || col0 + p.window > pos_last);
       const int hi_c = valid ? pos - col0 : -1, lo_c = (p.window > 0 ? pos - p.window + 1 : 0) - col0;     // columns the row sees
       const bool none = hi_c < lo_c;
@@ -543,7 +544,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
         l *= corr;
       }
       const float off = 12.f - (m == -INFINITY ? 0.f : m);
-      if (C::APART && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[x], (j - 1) & 1) && !abort_flag)) {
+      if (C::APART && j > 0 && !__all_sync(0xffffffffu, mbar_wait(&o_done[x], (j - 1) & 1))) {
         abort_flag = 1;                                        // (P and O of the tile before are read by its product until then)
         if (lane == 0) atomicExch(p.status, STATUS_TIMEOUT + 3);
         alive = false;
@@ -597,7 +598,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
           __syncwarp();
         }
       }
-      if (marks[j % META]) {
+      if (marked) {
         // values of the tile's pages that are NaN, for the keys that the row sees
         const uint32_t* at = snan + (size_t)(j % META) * KEYS * (HD / 32);
 #pragma unroll 1
