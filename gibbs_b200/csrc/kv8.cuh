@@ -104,16 +104,26 @@ static inline Step step_of(const GbPlanCtx* ctx) {
 // which stands for keys that nobody sees).
 __device__ __forceinline__ int page_id(const int* entry) { return (int)min((unsigned)*entry, 0x7fffffffu); }
 
-// Piece `index` of a launch over pieces of requests, `count(r)` for request r: which request (-1: none) and which of its
-// pieces.  A whole warp looks at 32 requests at a time; every lane gets the answer.  With `last_first` the requests are
-// taken from the last to the first.
+// A request of a step: its place, how many tokens it brings, how many it holds, and where in the step its tokens begin.
+struct Request {
+  int r, n, before, start;
+};
+// Piece `index` of a launch over pieces of requests, `count(n, before)` for a request: which request (r -1: none) and which of its
+// pieces.  A whole warp looks at 32 requests at a time, all that is known of them in one trip; every lane gets the answer.  With
+// `last_first` the requests are taken from the last to the first.
 template <typename Count>
-__device__ __forceinline__ int find_piece(int index, int n_requests, bool last_first, Count count, int& piece) {
+__device__ __forceinline__ Request find_piece(int index, const Step& step, bool last_first, Count count, int& piece) {
   const int lane = threadIdx.x & 31;
-  for (int base = 0; base < n_requests; base += 32) {
-    const int i = base + lane;
-    const int n = i < n_requests ? count(last_first ? n_requests - 1 - i : i) : 0;
-    int upto = n;
+  for (int base = 0; base < step.n_requests; base += 32) {
+    const int i = base + lane, r = last_first ? step.n_requests - 1 - i : i;
+    int n = 0, before = 0, start = 0, upto = 0;
+    if (i < step.n_requests) {
+      n = step.q_len[r];
+      before = step.start_pos[r];
+      start = step.q_start[r];
+      upto = count(n, before);
+    }
+    const int mine = upto;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
       const int v = __shfl_up_sync(0xffffffffu, upto, o);
@@ -122,12 +132,13 @@ __device__ __forceinline__ int find_piece(int index, int n_requests, bool last_f
     const unsigned have = __ballot_sync(0xffffffffu, index < upto);
     if (have) {
       const int who = __ffs(have) - 1;
-      piece = index - __shfl_sync(0xffffffffu, upto - n, who);
-      return last_first ? n_requests - 1 - (base + who) : base + who;
+      piece = index - __shfl_sync(0xffffffffu, upto - mine, who);
+      return {__shfl_sync(0xffffffffu, r, who), __shfl_sync(0xffffffffu, n, who), __shfl_sync(0xffffffffu, before, who),
+              __shfl_sync(0xffffffffu, start, who)};
     }
     index -= __shfl_sync(0xffffffffu, upto, 31);
   }
-  return -1;
+  return {-1, 0, 0, 0};
 }
 
 // The driver's cuTensorMapEncodeTiled (null where there is none).

@@ -34,20 +34,24 @@ template <int RT>
 __device__ __forceinline__ bool find_tile(const Attn& p, int index, Tile& t) {
   t.group = p.heads / p.kv_heads;
   int tile = 0;
-  if (p.step.one_each && t.group <= RT) {                      // (a tile a request: nothing to look for, a trip less)
-    t.r = p.step.n_requests - 1 - index;
+  Request q;
+  if (p.step.one_each && t.group <= RT) {                      // (a tile a request: nothing to look for)
+    q.r = p.step.n_requests - 1 - index;
+    q.n = p.step.q_len[q.r];
+    q.before = p.step.start_pos[q.r];
+    q.start = p.step.q_start[q.r];
   } else {
-    t.r = find_piece(index, p.step.n_requests, true,
-                     [&](int i) {
-                       const int rows = p.step.q_len[i] * t.group;
-                       return rows > p.few ? 0 : (rows + RT - 1) / RT;
-                     }, tile);
+    q = find_piece(index, p.step, true,
+                   [&](int n, int) {
+                     const int rows = n * t.group;
+                     return rows > p.few ? 0 : (rows + RT - 1) / RT;
+                   }, tile);
   }
-  if (t.r < 0) return false;
-  const int qlen = p.step.q_len[t.r];
-  t.qstart = p.step.q_start[t.r];
-  t.start = p.step.start_pos[t.r];
-  if (qlen <= 0) return false;
+  if (q.r < 0 || q.n <= 0) return false;
+  const int qlen = q.n;
+  t.r = q.r;
+  t.qstart = q.start;
+  t.start = q.before;
   const int tiles = (qlen * t.group + RT - 1) / RT;
   t.row0 = (tiles - 1 - tile) * RT;                            // the tiles with the most keys first
   t.rows = min(RT, qlen * t.group - t.row0);

@@ -134,15 +134,14 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   const int part = (int)blockIdx.x % p.parts, unit = (int)blockIdx.x / p.parts, kvh = unit % p.kv_heads;
 
   int tile = 0;
-  const int r = find_piece(unit / p.kv_heads, p.step.n_requests, true, [&](int i) {
-    const int n = p.step.q_len[i];
+  const Request q = find_piece(unit / p.kv_heads, p.step, true, [&](int n, int) {
     return n * group > p.few ? (n + 2 * tpt - 1) / (2 * tpt) : 0;
   }, tile);
-  if (r < 0) {                                                 // (the same for every CTA of a cluster)
+  if (q.r < 0) {                                               // (the same for every CTA of a cluster)
     if (p.second) pdl_wait();
     return;
   }
-  const int qlen = p.step.q_len[r], start = p.step.start_pos[r], qstart = p.step.q_start[r];
+  const int r = q.r, qlen = q.n, start = q.before, qstart = q.start;
   tile = (qlen + 2 * tpt - 1) / (2 * tpt) - 1 - tile;          // the tiles with the most keys first
   const int tok0 = tile * 2 * tpt, n_tok = min(2 * tpt, qlen - tok0);
   const int hi = start + tok0 + n_tok;                         // keys < hi may be visible

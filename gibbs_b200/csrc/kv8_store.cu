@@ -56,17 +56,17 @@ __global__ void __launch_bounds__(128) kv8_store_any_kernel(const Store p) {
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   int seg = 0;
-  const int r = find_piece((int)blockIdx.x, p.step.n_requests, false, [&](int i) {
-    const int n = p.step.q_len[i], b = p.step.start_pos[i];
-    return n > 0 ? (b + n - 1) / p.page_size - b / p.page_size + 1 : 0;
+  const Request q = find_piece((int)blockIdx.x, p.step, false, [&](int n, int before) {
+    return n > 0 ? (before + n - 1) / p.page_size - before / p.page_size + 1 : 0;
   }, seg);
+  const int r = q.r;
   const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
   const int slot = (int)blockIdx.y * 4 + warp;
   if (r < 0 || slot >= slots) return;
-  const int before = p.step.start_pos[r], end = before + p.step.q_len[r];
+  const int before = q.before, end = before + q.n;
   const int block = before / p.page_size + seg;
   const int from = max(before, block * p.page_size), to = min(end, (block + 1) * p.page_size);      // positions of the unit
-  const int row0 = p.step.q_start[r] + (from - before);
+  const int row0 = q.start + (from - before);
   const int hd = p.hd;
   const bool is_q = slot < p.heads, is_k = !is_q && slot < p.heads + p.kv_heads;
   const int kvh = is_q ? 0 : (slot - p.heads) % p.kv_heads;
@@ -346,15 +346,15 @@ __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) kv8_store_pages_kernel(
   pdl_trigger();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, sub = lane % TPR;
   int seg = 0;
-  const int r = find_piece((int)blockIdx.x, p.step.n_requests, false, [&](int i) {
-    const int n = p.step.q_len[i], b = p.step.start_pos[i];
-    return n > 0 ? (b + n - 1) / p.page_size - b / p.page_size + 1 : 0;
+  const Request q = find_piece((int)blockIdx.x, p.step, false, [&](int n, int before) {
+    return n > 0 ? (before + n - 1) / p.page_size - before / p.page_size + 1 : 0;
   }, seg);
+  const int r = q.r;
   if (r < 0) return;
-  const int before = p.step.start_pos[r], end = before + p.step.q_len[r];
+  const int before = q.before, end = before + q.n;
   const int block = before / p.page_size + seg, base = block * p.page_size;
   const int from = max(before, base) - base, to = min(end, base + p.page_size) - base;      // new rows of the page
-  const int row0 = p.step.q_start[r] + base - before;                   // batch row of the page's row 0 (if it were new)
+  const int row0 = q.start + base - before;                   // batch row of the page's row 0 (if it were new)
   const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
   const int wpu = p.page_size / 16, wu = warp % wpu, units = 8 / wpu;
   int page = -1;
