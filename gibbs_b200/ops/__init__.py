@@ -66,7 +66,7 @@ def raw_stream(device: torch.device) -> int:
     ``launching_on`` block is active for)."""
     if _STREAM is not None:
         return _STREAM.value or 0
-    index = torch.cuda.current_device()
+    index = torch._C._cuda_getDevice()             # (the tensors are CUDA tensors: CUDA is initialised)
     if device.index != index:
         raise KernelError(f"the tensors lie on {device}, the current device is cuda:{index}")
     return torch._C._cuda_getCurrentRawStream(index)

@@ -121,13 +121,13 @@ def _is(ok: bool, message: str) -> None:
 # The checks of a call are made twice over: as one expression, which is what a good call costs (a decode step makes a dozen of
 # them), and one by one with their messages where that expression is false.
 
-def _step_ok(step, block_table, page_size: int, rows: int, index: int) -> bool:
+def _step_ok(step, block_table, table, page_size: int, rows: int, index: int) -> bool:
     n, a, b, c = step.n_requests, step.q_start, step.q_len, step.start_pos
     return (a.dtype is _I32 and b.dtype is _I32 and c.dtype is _I32 and a.get_device() == index and b.get_device() == index
             and c.get_device() == index and a.is_contiguous() and b.is_contiguous() and c.is_contiguous() and a.numel() >= n
             and b.numel() >= n and c.numel() >= n and block_table.dtype is _I32 and block_table.get_device() == index
-            and block_table.dim() == 2 and block_table.is_contiguous() and block_table.shape[0] >= n and rows >= step.n_tokens
-            and block_table.shape[1] * page_size >= step.max_ctx_len)
+            and len(table) == 2 and block_table.is_contiguous() and table[0] >= n and rows >= step.n_tokens
+            and table[1] * page_size >= step.max_ctx_len)
 
 
 def _refuse_step(step, block_table, page_size: int, rows: int, index: int, what: str) -> None:
@@ -159,6 +159,7 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
     index, cols = x.get_device(), (heads + (2 * kv_heads if pages is not None else 0)) * head_dim
     if inv_freq is not None and inv_freq.numel() != rotary_dim // 2 + 1 and not rotary_dim % 2:
         inv_freq = _rotary_table(inv_freq, rotary_dim)
+    table, outs = block_table.shape, q_out.shape
     if part is None:
         shape, stride = x.shape, x.stride()
         good = len(shape) == 2 and (stride[1] == 1 or shape[1] == 1) and shape[1] >= cols and (x.dtype is _BF16 or x.dtype is _F32)
@@ -168,12 +169,12 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
         good = (x.dtype is _F32 and x.is_contiguous() and x.dim() == 3 and tuple(x.shape[1:]) == (rows, cols)
                 and part.dtype is _BF16 and _vector_ok(part.bias, cols, index))
     if not (good and index >= 0 and heads > 0 and kv_heads > 0 and not head_dim % 8 and 8 <= head_dim <= MAX_HEAD_DIM
-            and q_out.dtype is dtype and q_out.get_device() == index and q_out.dim() == 2 and q_out.shape[1] == heads * head_dim
-            and q_out.shape[0] >= step.n_tokens and q_out.is_contiguous() and _vector_ok(q_gain, head_dim, index)
+            and q_out.dtype is dtype and q_out.get_device() == index and len(outs) == 2 and outs[1] == heads * head_dim
+            and outs[0] >= step.n_tokens and q_out.is_contiguous() and _vector_ok(q_gain, head_dim, index)
             and _vector_ok(k_gain, head_dim, index) and (inv_freq is None or (
                 not rotary_dim % 2 and 0 <= rotary_dim <= head_dim and _vector_ok(inv_freq, rotary_dim // 2 + 1, index)))
             and (pages is None or (pages.kv_heads == kv_heads and pages.head_dim == head_dim and pages.index == index))
-            and _step_ok(step, block_table, 1 << 40 if pages is None else pages.page_size, rows, index)):
+            and _step_ok(step, block_table, table, 1 << 40 if pages is None else pages.page_size, rows, index)):
         _refuse_store(x, part, good, rows, cols, q_out, heads, kv_heads, head_dim, q_gain, k_gain, inv_freq, rotary_dim, step,
                       block_table, pages, index, dtype)
     if pages is not None:
@@ -186,7 +187,7 @@ def qk_norm_rope_store(qkv, q_out: torch.Tensor, heads: int, kv_heads: int, head
         x.data_ptr() if part is None else 0, ld, BF16 if dtype is _BF16 else F32, q_out.data_ptr(),
         0 if q_gain is None else q_gain.data_ptr(), 0 if k_gain is None else k_gain.data_ptr(),
         0 if inv_freq is None else inv_freq.data_ptr(), 0 if inv_freq is None else rotary_dim, 1 if adjacent_pairs else 0, k, v, ks,
-        vs, n_pages, page_size, heads, kv_heads, head_dim, block_table.data_ptr(), block_table.shape[1]), eps, step, part)
+        vs, n_pages, page_size, heads, kv_heads, head_dim, block_table.data_ptr(), table[1]), eps, step, part)
     return q_out
 
 
@@ -216,15 +217,16 @@ def paged_attention(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, p
     wider row.  ``window`` 0: none; block tables hold the step's longest context.  Rows of ``out`` behind the step's tokens are left as
     they are."""
     index, cols, qs, os_, dtype = q.get_device(), heads * head_dim, q.stride(), out.stride(), q.dtype
+    table, rows, outs = block_table.shape, q.shape, out.shape
     if not (index >= 0 and heads > 0 and kv_heads > 0 and not heads % kv_heads and len(qs) == 2 and len(os_) == 2
-            and q.shape[1] == cols and out.shape[1] == cols and (qs[1] == 1 or cols == 1) and (os_[1] == 1 or cols == 1)
-            and out.dtype is dtype and (dtype is _BF16 or dtype is _F32) and out.shape[0] >= step.n_tokens and out.get_device() == index
+            and rows[1] == cols and outs[1] == cols and (qs[1] == 1 or cols == 1) and (os_[1] == 1 or cols == 1)
+            and out.dtype is dtype and (dtype is _BF16 or dtype is _F32) and outs[0] >= step.n_tokens and out.get_device() == index
             and pages.kv_heads == kv_heads and pages.head_dim == head_dim and pages.index == index and window is not None and window >= 0
-            and (os_[0] >= cols or out.shape[0] == 1) and _step_ok(step, block_table, pages.page_size, q.shape[0], index)):
+            and (os_[0] >= cols or outs[0] == 1) and _step_ok(step, block_table, table, pages.page_size, rows[0], index)):
         _refuse_attention(q, heads, kv_heads, head_dim, pages, block_table, window, out, step, index)
     k, v, ks, vs = pages.addresses
     _call(1, index, q.device, (q.data_ptr(), qs[0], BF16 if dtype is _BF16 else F32, out.data_ptr(), os_[0], k, v, ks, vs, pages.n_pages,
-                               pages.page_size, heads, kv_heads, head_dim, block_table.data_ptr(), block_table.shape[1], window, 0, 0, 0),
+                               pages.page_size, heads, kv_heads, head_dim, block_table.data_ptr(), table[1], window, 0, 0, 0),
           scale, step)
     return out
 
