@@ -443,7 +443,7 @@ __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
 // rows by the 16-byte piece XOR row, 64-byte rows by piece XOR row / 2) and the keys of a group take the places pi(0..15) of the
 // products: with these every fragment is read without a bank conflict.
 // Bound by memory and by how evenly the CTAs lie on the SMs: 64 requests of 2,112 keys, 32 / 8 heads of 64, 30.3 us, 4.6 TB/s of the
-// cache's 139 MB; 4 requests of 30,000 to 32,768 keys, 32 / 8 heads of 128, 48.0 us, 5.4 TB/s; one request of 2,048 keys 7.3 us, by its trips.
+// cache's 139 MB; 4 requests of 30,000 to 32,768 keys, 32 / 8 heads of 128, 47.3 us, 5.4 TB/s; one request of 2,048 keys 7.3 us, by its trips.
 template <int HD, int WARPS> struct Mma {
   static constexpr int NW = WARPS;
   static constexpr int NG = 2;                                 // groups of a slot, taken together

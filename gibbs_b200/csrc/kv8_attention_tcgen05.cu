@@ -11,13 +11,13 @@
 //                weights in f16 to tensor memory, from where they are the A operand of the second product
 //
 // The two row tiles take turns: while one is in its softmax the other's products run, and both use the same converted K and V.  (Products
-// issued as either tile is ready, without that order: 48 us against 47 at 2,048 tokens, 345 against 326 at 8,192.)
+// issued as either tile is ready, without that order: 48 us against 47 at 2,048 tokens, 345 against 327 at 8,192.)
 //
-// 2,048 tokens, 32 / 8 heads of 64: 47 us, 366 TFLOP/s; 8,192 tokens, 16 / 4 heads of 128: 320 us, 858 TFLOP/s.  What bounds it, from copies
-// that leave work out: heads of 64 take 45 us without the 2^x, 40 without any softmax, 34 without conversion and loads either, so it is
+// 2,048 tokens, 32 / 8 heads of 64: 44.8 us, 384 TFLOP/s; 8,192 tokens, 16 / 4 heads of 128: 315 us, 873 TFLOP/s.  What bounds it, from
+// copies that left work out when it took 47 and 327: heads of 64 take 45 us without the 2^x, 40 without any softmax, 34 without conversion and loads either, so it is
 // the hand-overs of a key tile (scores to registers, weights back, product) and a CTA's beginning and end; heads of 128 take 301 us
 // without conversion, 296 without softmax and 229 without both.  The special-function unit is at 37 % (a share of the 2^x by a
-// polynomial is slower: 49 and 341 us).
+// polynomial is slower: 49 and 341 us).  Weights go over in halves: whole they take 51 us, in quarters 50.
 //
 // Scales, as in the kernel for few rows: q's row under the power of two that brings its largest magnitude to 2^14; a score
 // times the inverse and the scale of K's page; the scale of V's page in the exponent, x_j = score_j + log2(scale_j), weights
