@@ -518,8 +518,9 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   __syncwarp();
 
   // The warp's groups are numbered n = 0, 1, ... (chunk n / NG).  Lane i holds what belongs to group 32 b + i: the row of its
-  // first key in the pool (NONE where nothing of it is visible: no page has it, and none of its keys counts), and the page's scales.
-  constexpr int NONE = -1;
+  // first key in the pool (ABSENT where nothing of it is visible: no page has it, and none of its keys counts), and the page's scales.
+  constexpr int NONE = -1;                                     // (a page)
+  constexpr int ABSENT = -16;                                  // (a group: sixteen rows in front of the pool, which a copy fills with zeros)
   auto page_of = [&](int n) {
     const int c = first + (n / NG) * stride, j = (c_lo + c) * CK + (n % NG) * 16;
     return (c >= chunks || j >= t.hi || j + 15 < t.lo) ? NONE : page_id(bt + (j >> p.page_shift));
@@ -531,7 +532,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   };
   auto row_of = [&](int n, int page) {
     const int j = (c_lo + first + (n / NG) * stride) * CK + (n % NG) * 16;
-    return page == NONE ? NONE : (((page * p.kv_heads + kvh) << p.page_shift) | (j & (p.page_size - 1)));
+    return page == NONE ? ABSENT : (((page * p.kv_heads + kvh) << p.page_shift) | (j & (p.page_size - 1)));
   };
   // Requests run SLOTS chunks ahead of the products: `row` is of the 32 groups that are being requested, `ks`, `vs` of the 32 that
   // are being worked on, `ks_next`, `vs_next` of the former where they differ, `page_ahead` of the 32 behind those.
@@ -547,11 +548,12 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
     }
   };
   uint8_t* ring = smem + warp * SLOTS * C::SLOT;
-  // Requests the groups of the warp's chunk i.  A group without a page brings row 0 of the pool, which is never looked at.
+  // Requests the groups of the warp's chunk i.  A group without a page comes as zeros: its weights are 0, and 0 times what a page of
+  // another request holds need not be 0.
   auto request = [&](int i, int slot) {
     int at[NG];
 #pragma unroll
-    for (int y = 0; y < NG; ++y) at[y] = max(0, __shfl_sync(0xffffffffu, row, (i * NG + y) & 31));
+    for (int y = 0; y < NG; ++y) at[y] = __shfl_sync(0xffffffffu, row, (i * NG + y) & 31);
     if (lane == 0) {
       uint8_t* dst = ring + slot * C::SLOT;
       sm100::mbar_arrive_expect_tx(&full[warp][slot], C::SLOT);
