@@ -9,7 +9,7 @@
 //
 // a0 q rows, a1 their stride, a2 dtype (of q and out), a3 out, a4 its stride, a5 k pages, a6 v pages, a7 k scales, a8 v
 // scales, a9 pages, a10 page size, a11 heads, a12 kv heads, a13 hd, a14 block table, a15 its stride, a16 window (0: none);
-// f0 scale.  The step's requests come from its symbols.
+// f0 scale (of any sign, finite).  The step's requests come from its symbols.
 #include "kv8_attention.cuh"
 
 namespace {
@@ -959,6 +959,7 @@ GB_OP(gb_op_kv8_attention) {
     GB_FAIL(GB_ERR_ARG, "kv8_attention: %d heads, %d kv heads, head_dim %d, pages of %d: head sizes are multiples of 8 up to 256",
             p.heads, p.kv_heads, p.hd, p.page_size);
   if (dtype != GB_F32 && dtype != GB_BF16) GB_FAIL(GB_ERR_ARG, "kv8_attention: q and out are float32 or bfloat16");
+  if (!isfinite(p.scale_log2)) GB_FAIL(GB_ERR_ARG, "kv8_attention: a scale of %g", f[0]);
   const int group = p.heads / p.kv_heads;
   p.page_shift = 0;
   while ((1 << p.page_shift) < p.page_size) ++p.page_shift;

@@ -450,8 +450,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     const bool valid = row / group < tpt && tl < n_tok;
     const int pos = first + tl, pos_first = first + x * tpt, pos_last = first + min(n_tok, (x + 1) * tpt) - 1;
     const uint32_t lane_off = (uint32_t)(32 * (warp & 3)) << 16;
-    // q under its power of two, in f16
-    float factor;                                              // scale * log2(e) / that power
+    // q under its power of two, in f16, and under the sign of the scale: the factor of the scores is not negative, so the largest
+    // score of a group of keys is the largest under its factor too
+    float factor;                                              // |scale| * log2(e) / that power
     {
       uint4 w[HD / 8];
       const uint4* src = reinterpret_cast<const uint4*>(reinterpret_cast<const bf16*>(p.q) + (size_t)(qstart + tok0 + tl) * p.ldq +
@@ -469,8 +470,8 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
         for (int e = 0; e < 4; ++e) top = max(top, max(u[e] & 0x7fffu, (u[e] >> 16) & 0x7fffu));
       }
       const int e2 = min(127, max((int)(top >> 7) - 127, -112));
-      const float up = pow2(min(14 - e2, 126));
-      factor = p.scale_log2 * pow2(max(e2 - 14, -126));
+      const float up = copysignf(pow2(min(14 - e2, 126)), p.scale_log2);
+      factor = fabsf(p.scale_log2) * pow2(max(e2 - 14, -126));
       uint8_t* dst = sq + (size_t)x * C::Q_TILE + (size_t)row * 128;
 #pragma unroll
       for (int i = 0; i < HD / 8; ++i) {

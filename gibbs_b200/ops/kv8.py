@@ -214,8 +214,8 @@ def _refuse_store(x, part, good, rows, cols, q_out, heads, kv_heads, head_dim, q
 def paged_attention(q: torch.Tensor, heads: int, kv_heads: int, head_dim: int, pages: Pages, block_table: torch.Tensor,
                     scale: float, window: int, out: torch.Tensor, step) -> torch.Tensor:
     """out[t, h, :] = softmax over visible keys of (q.K)*scale, times V, over an 8-bit cache; q may be a column slice of a
-    wider row.  ``window`` 0: none; block tables hold the step's longest context.  Rows of ``out`` behind the step's tokens are left as
-    they are."""
+    wider row.  ``scale``: finite, of any sign.  ``window`` 0: none; block tables hold the step's longest context.  Rows of
+    ``out`` behind the step's tokens are left as they are."""
     index, cols, qs, os_, dtype = q.get_device(), heads * head_dim, q.stride(), out.stride(), q.dtype
     table, rows, outs = block_table.shape, q.shape, out.shape
     if not (index >= 0 and heads > 0 and kv_heads > 0 and not heads % kv_heads and len(qs) == 2 and len(os_) == 2

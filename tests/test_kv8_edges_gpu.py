@@ -1,5 +1,6 @@
 """The 8-bit paged cache where its kernels meet what is not theirs: pages of other requests, the way from kernel to kernel, the
 values of an argument at the ends of its range.  One way through every kernel each."""
+import math
 import random
 
 import pytest
@@ -53,3 +54,45 @@ def test_nan_in_pages_that_a_request_does_not_hold(way, window):
         got = call()
         assert int(step.status.item()) == 0 and not bool(got.isnan().any())
         assert torch.equal(got, want)
+@pytest.mark.parametrize("way", WAYS)
+def test_scales_below_zero_and_zero(way):
+    """softmax(-s q K^T) V is that of -q under s, to the bit; under 0 every visible key has the same weight."""
+    from gibbs_b200.ops import kv8
+    dtype, heads, kv_heads, hd, page, portions = WAYS[way]
+    behind = [(37 * i) % 90 for i in range(len(portions))]
+    gen = torch.Generator().manual_seed(2)
+    n_pages, bt = tables(portions, behind, page, random.Random(1))
+    pages = make_pages(n_pages, kv_heads, page, hd, gen)
+    q = torch.randn(sum(portions), heads * hd, generator=gen).to(dtype).to(DEV)
+    call = lambda x, scale: kv8.paged_attention(x, heads, kv_heads, hd, pages, bt.to(DEV), scale, 0, torch.empty_like(q),  # noqa: E731
+                                                step_of(portions, behind))
+    assert torch.equal(call(q, -0.3), call(-q, 0.3)) and not torch.equal(call(q, -0.3), call(q, 0.3))
+    got = call(q, 0.0).double().cpu().view(-1, kv_heads, heads // kv_heads, hd)
+    values, row = pages.dequantized()[1].double().cpu(), 0
+    for r, (p, b) in enumerate(zip(portions, behind)):
+        n = b + p
+        ids = bt[r, :-(-n // page)].long()
+        for h in range(kv_heads):
+            v = values[ids, h].reshape(-1, hd)[:n]
+            upto = torch.arange(b + 1, n + 1).double()[:, None]
+            want, weight = v.cumsum(0)[b:] / upto, v.abs().cumsum(0)[b:] / upto
+            # 32-bit sums over n keys (2^-23 of their magnitudes each) and a quotient; in 16 bits a weight's rounding (2^-11 of it),
+            # 2^-37 * 448 * (keys) * (the largest page scale over the keys) where a weight is that small, and the output's own (2^-8)
+            tol = (n + 64) * 2.0 ** -23 * weight
+            if dtype == torch.bfloat16:
+                most = (pages.v_scales[ids.to(DEV), h].abs().max().item())
+                tol = tol + 2.0 ** -11 * weight + 2.0 ** -37 * 448 * most + 2.0 ** -8 * want.abs()
+            assert bool(((got[row:row + p, h] - want[:, None]).abs() <= tol[:, None]).all())
+        row += p
+
+
+@pytest.mark.parametrize("scale", [math.nan, math.inf, -math.inf, 1e39])
+def test_scales_that_are_not_finite_are_refused(scale):
+    from gibbs_b200.ops import KernelError, kv8
+    for way in ("8 rows, 64", "256 rows, 64", "32 bits"):
+        dtype, heads, kv_heads, hd, page, portions = WAYS[way]
+        n_pages, bt = tables(portions, [0] * len(portions), page, random.Random(1))
+        pages = make_pages(n_pages, kv_heads, page, hd, torch.Generator().manual_seed(2))
+        q = torch.zeros(sum(portions), heads * hd, dtype=dtype, device=DEV)
+        with pytest.raises(KernelError, match="scale"):
+            kv8.paged_attention(q, heads, kv_heads, hd, pages, bt.to(DEV), scale, 0, torch.empty_like(q), step_of(portions, [0] * len(portions)))
