@@ -141,6 +141,12 @@ __device__ __forceinline__ Request find_piece(int index, const Step& step, bool 
   return {-1, 0, 0, 0};
 }
 
+// Before a block without work leaves: the first one of a launch waits like those that work, so that a launch all of whose blocks leave
+// still ends behind the kernel in front (what comes next waits for this launch alone).
+__device__ __forceinline__ void leave() {
+  if (blockIdx.x == 0 && blockIdx.y == 0) pdl_wait();
+}
+
 // The driver's cuTensorMapEncodeTiled (null where there is none).
 typedef CUresult (*TensorMapFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
                                 const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,

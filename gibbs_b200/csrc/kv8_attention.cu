@@ -136,7 +136,7 @@ __global__ void __launch_bounds__(128) kv8_attention_any_kernel(const Attn p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, hd = p.hd;
   const int part = (int)blockIdx.x % p.parts, unit = (int)blockIdx.x / p.parts, kvh = unit % p.kv_heads;
   Tile t;
-  if (!find_tile<RT>(p, unit / p.kv_heads, t)) return;          // (the same for every CTA of a cluster)
+  if (!find_tile<RT>(p, unit / p.kv_heads, t)) return leave();  // (the same for every CTA of a cluster)
   const int c_lo = t.lo / 32, chunks = (t.hi + 31) / 32 - c_lo;
   const int parts = max(1, min(p.parts, (chunks + NW - 1) / NW));
   if (part >= parts) return;                                   // (a thread that has left counts as arrived at the cluster's barriers)
@@ -272,7 +272,7 @@ __global__ void __launch_bounds__(128) kv8_attention_rows_kernel(const Attn p) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, db = lane % LPR, kg = lane / LPR;
   const int part = (int)blockIdx.x % p.parts, unit = (int)blockIdx.x / p.parts, kvh = unit % p.kv_heads;
   Tile t;
-  if (!find_tile<RT>(p, unit / p.kv_heads, t)) return;         // (the same for every CTA of a cluster)
+  if (!find_tile<RT>(p, unit / p.kv_heads, t)) return leave();  // (the same for every CTA of a cluster)
   const int c_lo = t.lo / 32, chunks = (t.hi + 31) / 32 - c_lo;
   const int parts = max(1, min(p.parts, (chunks + NW - 1) / NW));
   if (part >= parts) return;                                   // (a thread that has left counts as arrived at the cluster's barriers)
@@ -504,7 +504,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const int parts = max(1, min(p.parts, (chunks + NW - 1) / NW));
   if (!found || part >= parts) {                               // (a thread that has left counts as arrived at the cluster's barriers)
     if (p.first) pdl_wait();
-    return;
+    return leave();
   }
   const int* bt = p.block_table + (size_t)t.r * p.bt_stride;
   const int stride = parts * NW, first = part * NW + warp;

@@ -139,7 +139,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   }, tile);
   if (q.r < 0) {                                               // (the same for every CTA of a cluster)
     if (p.second) pdl_wait();
-    return;
+    return leave();
   }
   const int r = q.r, qlen = q.n, start = q.before, qstart = q.start;
   tile = (qlen + 2 * tpt - 1) / (2 * tpt) - 1 - tile;          // the tiles with the most keys first

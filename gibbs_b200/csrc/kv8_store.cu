@@ -62,7 +62,7 @@ __global__ void __launch_bounds__(128) kv8_store_any_kernel(const Store p) {
   const int r = q.r;
   const int slots = p.heads + (p.write ? 2 * p.kv_heads : 0);
   const int slot = (int)blockIdx.y * 4 + warp;
-  if (r < 0 || slot >= slots) return;
+  if (r < 0 || slot >= slots) return leave();
   const int before = q.before, end = before + q.n;
   const int block = before / p.page_size + seg;
   const int from = max(before, block * p.page_size), to = min(end, (block + 1) * p.page_size);      // positions of the unit
@@ -269,7 +269,7 @@ __global__ void __launch_bounds__(128) kv8_store_rows_kernel(const Store p) {
   const bool active = slot < slots;
   const bool is_q = slot < p.heads, is_k = !is_q && slot < p.heads + p.kv_heads;
   const int pos = p.step.start_pos[r], row = p.step.q_start[r];
-  if (p.step.q_len[r] <= 0) return;                            // (the whole block)
+  if (p.step.q_len[r] <= 0) return leave();                    // (the whole block)
   int page = -1;
   if (active && !is_q) page = p.block_table[(size_t)r * p.bt_stride + pos / p.page_size];
   const int held = pos % p.page_size;                          // rows that the page holds already
@@ -350,7 +350,7 @@ __global__ void __launch_bounds__(256, HD == 64 ? 3 : 2) kv8_store_pages_kernel(
     return n > 0 ? (before + n - 1) / p.page_size - before / p.page_size + 1 : 0;
   }, seg);
   const int r = q.r;
-  if (r < 0) return;
+  if (r < 0) return leave();
   const int before = q.before, end = before + q.n;
   const int block = before / p.page_size + seg, base = block * p.page_size;
   const int from = max(before, base) - base, to = min(end, base + p.page_size) - base;      // new rows of the page

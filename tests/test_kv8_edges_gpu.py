@@ -96,3 +96,29 @@ def test_scales_that_are_not_finite_are_refused(scale):
         q = torch.zeros(sum(portions), heads * hd, dtype=dtype, device=DEV)
         with pytest.raises(KernelError, match="scale"):
             kv8.paged_attention(q, heads, kv_heads, hd, pages, bt.to(DEV), scale, 0, torch.empty_like(q), step_of(portions, [0] * len(portions)))
+
+
+def test_a_launch_without_work_ends_behind_the_kernel_in_front():
+    """Requests without tokens (a padded step's): nothing is read or written, and what comes next still waits for what came before."""
+    from gibbs_b200.ops import kv8
+    gen = torch.Generator().manual_seed(4)
+    for way in WAYS:
+        dtype, heads, kv_heads, hd, page, portions = WAYS[way]
+        n_pages, bt = tables(portions, [40] * len(portions), page, random.Random(1))
+        pages, bt = make_pages(n_pages, kv_heads, page, hd, gen), bt.to(DEV)
+        before = [bits(t).clone() for t in pages.tensors()]
+        step, none = (step_of(portions, [40] * len(portions)) for _ in range(2))
+        none.q_len = torch.zeros_like(none.q_len)
+        n = sum(portions)
+        x = torch.randn(n, (heads + 2 * kv_heads) * hd, generator=gen).to(dtype).to(DEV)
+        q, out = (torch.full((n, heads * hd), 7.0, dtype=dtype, device=DEV) for _ in range(2))
+        kv8.qk_norm_rope_store(x, q, heads, kv_heads, hd, None, None, 1e-5, None, 0, False, none, bt, pages)
+        kv8.paged_attention(q, heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, out, none)
+        assert bool((q == 7.0).all()) and bool((out == 7.0).all())
+        assert all(torch.equal(bits(a), b) for a, b in zip(pages.tensors(), before))
+        kv8.qk_norm_rope_store(x, q, heads, kv_heads, hd, None, None, 1e-5, None, 0, False, step, bt, pages)
+        kv8.paged_attention(torch.zeros_like(q), heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, out, none)
+        got = kv8.paged_attention(q, heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, torch.empty_like(q), step)
+        torch.cuda.synchronize()
+        assert torch.equal(got, kv8.paged_attention(q, heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, out, step))
+        assert int(step.status.item()) == 0
