@@ -502,10 +502,7 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   const bool found = find_tile<RT>(p, unit / p.kv_heads, t);   // (the same for every CTA of a cluster)
   const int c_lo = found ? t.lo / CK : 0, chunks = found ? (t.hi + CK - 1) / CK - c_lo : 0;
   const int parts = max(1, min(p.parts, (chunks + NW - 1) / NW));
-  if (!found || part >= parts) {                               // (a thread that has left counts as arrived at the cluster's barriers)
-    if (p.first) pdl_wait();
-    return leave();
-  }
+  if (!found || part >= parts) return leave();                 // (a thread that has left counts as arrived at the cluster's barriers)
   const int* bt = p.block_table + (size_t)t.r * p.bt_stride;
   const int stride = parts * NW, first = part * NW + warp;
   const int mine = first < chunks ? (chunks - 1 - first) / stride + 1 : 0;           // chunks of this warp
@@ -567,7 +564,6 @@ kv8_attention_mma_kernel(const __grid_constant__ CUtensorMap map_k, const __grid
   gb_pin(row);
   gb_pin(page_ahead);
   pdl_wait();
-  if (p.first) pdl_trigger();
 #pragma unroll
   for (int i = 0; i < SLOTS; ++i)
     if (i < mine) request(i, i);
@@ -969,16 +965,12 @@ GB_OP(gb_op_kv8_attention) {
   // Requests of more than FEW rows go to tcgen05, which takes 256 rows at a time; they have to lie on 16-byte boundaries.
   const bool wide = mma && (long long)p.step.max_q * group > FEW && group <= 64 && p.ldo % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
   p.few = 0x7fffffff;
-  p.first = p.second = 0;
   if (wide && p.step.n_requests == 1) {
     p.few = 0;                                                 // (all of it, whatever it brings)
     const int rc = kv8_attention_tcgen05(p, ctx->stream);
     return rc == GB_OK ? 1 : rc;
   }
-  if (wide) {
-    p.few = FEW;
-    p.first = 1;
-  }
+  if (wide) p.few = FEW;
   // upper bound of the tiles: sum_r ceil(q_len_r * group / rt)
   auto tiles_of = [&](int rt) {
     return p.step.one_each ? (long long)p.step.n_requests * ((group + rt - 1) / rt)
@@ -1005,8 +997,8 @@ GB_OP(gb_op_kv8_attention) {
   if (rc != GB_OK) return rc;
   GB_CHECK_LAUNCH("kv8_attention");
   if (!wide) return 1;
-  p.first = 0;
-  p.second = 1;
+  // (The second launch waits for the first, like any kernel for the one in front: what the kernels before them wrote is sure to be seen
+  // only behind a launch's own wait.)
   rc = kv8_attention_tcgen05(p, ctx->stream);
   return rc == GB_OK ? 2 : rc;
 }

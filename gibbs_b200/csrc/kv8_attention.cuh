@@ -15,10 +15,6 @@ struct Attn {
   int parts;                         // CTAs of a cluster
   int page_shift;                    // log2 of the page size, where that is a power of two
   int few;                           // a launch's requests: of more than `few` rows (tcgen05), of `few` at most (mma.sync)
-  // Two launches of one step, for requests of few rows and for the others, run beside each other: the first lets the second start as
-  // soon as what both read is in place (`first`: every CTA of it waits for that), and the second waits for the first to end before it
-  // ends itself (`second`), so that whatever comes behind the two finds both done.
-  int first, second;
   float scale_log2;                  // scale * log2(e)
   int* status;
 };

@@ -137,10 +137,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   const Request q = find_piece(unit / p.kv_heads, p.step, true, [&](int n, int) {
     return n * group > p.few ? (n + 2 * tpt - 1) / (2 * tpt) : 0;
   }, tile);
-  if (q.r < 0) {                                               // (the same for every CTA of a cluster)
-    if (p.second) pdl_wait();
-    return leave();
-  }
+  if (q.r < 0) return leave();                                 // (the same for every CTA of a cluster)
   const int r = q.r, qlen = q.n, start = q.before, qstart = q.start;
   tile = (qlen + 2 * tpt - 1) / (2 * tpt) - 1 - tile;          // the tiles with the most keys first
   const int tok0 = tile * 2 * tpt, n_tok = min(2 * tpt, qlen - tok0);
@@ -149,10 +146,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   const int lo = (p.window > 0 && first - p.window + 1 > 0) ? first - p.window + 1 : 0;
   int t_lo = lo / KEYS, t_hi = (hi + KEYS - 1) / KEYS;
   const int parts = max(1, min(p.parts, (t_hi - t_lo) / 2));
-  if (part >= parts) {                                         // (a thread that has left counts as arrived at the cluster's barriers)
-    if (p.second) pdl_wait();
-    return;
-  }
+  if (part >= parts) return;                                   // (a thread that has left counts as arrived at the cluster's barriers)
   {
     const int whole = t_hi - t_lo, from = t_lo;
     t_lo = from + whole * part / parts;
@@ -190,7 +184,7 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   const uint32_t tmem = tmem_slot;
   const uint32_t tmem_s[2] = {tmem, tmem + KEYS}, tmem_o[2] = {tmem + 2 * KEYS, tmem + 2 * KEYS + HD};
   const uint32_t tmem_p[2] = {C::APART ? tmem + 2 * KEYS + 2 * HD : tmem, C::APART ? tmem + 2 * KEYS + 2 * HD + KEYS / 2 : tmem + KEYS};
-  if (!p.second) pdl_wait();
+  pdl_wait();
 
   if (warp >= 8 && warp < 11) {
     // ---- K and V: pages -> f16 tiles ----
@@ -699,7 +693,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
       for (int i = 0; i < 1000; ++i) __nanosleep(1000);        // products still on their way end before their memory is given back
     tmem_dealloc(tmem_slot, 512);
   }
-  if (p.second) pdl_wait();
 }
 
 constexpr int MAX_SHARES = 8;

@@ -98,6 +98,39 @@ def test_scales_that_are_not_finite_are_refused(scale):
             kv8.paged_attention(q, heads, kv_heads, hd, pages, bt.to(DEV), scale, 0, torch.empty_like(q), step_of(portions, [0] * len(portions)))
 
 
+@pytest.mark.parametrize("way", WAYS)
+def test_store_and_attention_one_right_behind_the_other(way):
+    """A step's store and attention launched without a pause, over other rows every time: each sees what the kernel in front wrote."""
+    from gibbs_b200.ops import kv8
+    dtype, heads, kv_heads, hd, page, portions = WAYS[way]
+    behind = [(37 * i) % 90 for i in range(len(portions))]
+    gen = torch.Generator().manual_seed(3)
+    n_pages, bt = tables(portions, behind, page, random.Random(1))
+    clean = make_pages(n_pages, kv_heads, page, hd, gen)
+    rows = [torch.randn(sum(portions), (heads + 2 * kv_heads) * hd, generator=gen).to(dtype).to(DEV) for _ in range(8)]
+    bt, step = bt.to(DEV), step_of(portions, behind)
+
+    def run(pause):
+        pages = kv8.Pages(*(t.clone() for t in clean.tensors()))
+        outs = []
+        torch.cuda.synchronize()
+        for x in rows:
+            q, out = (torch.empty(sum(portions), heads * hd, dtype=dtype, device=DEV) for _ in range(2))
+            for _ in range(2):                                     # (the second over the first's pages, which lets the host run ahead)
+                kv8.qk_norm_rope_store(x, q, heads, kv_heads, hd, None, None, 1e-5, None, 0, False, step, bt, pages)
+                pause()
+                kv8.paged_attention(q, heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, out, step)
+                pause()
+            outs.append(out)
+        return outs
+
+    want = run(torch.cuda.synchronize)
+    for _ in range(5):
+        for a, b in zip(run(lambda: None), want):
+            assert torch.equal(a, b)
+    assert int(step.status.item()) == 0
+
+
 def test_a_launch_without_work_ends_behind_the_kernel_in_front():
     """Requests without tokens (a padded step's): nothing is read or written, and what comes next still waits for what came before."""
     from gibbs_b200.ops import kv8
