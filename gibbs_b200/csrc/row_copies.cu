@@ -4,8 +4,8 @@
 //
 // The tensors' rows are cut into pieces of at most 4 KB once, when the cache is made; a warp moves one piece of one pair, in
 // one trip (eight 16-byte loads a lane in flight).  The pairs travel in the launch's arguments: no copy to the device goes in
-// front.  Bound by memory: every byte is read once and written once; 1,000 pages of twelve tensors, 197 MB in and out, 36.4 us, 5.4
-// TB/s.  One page and a state slot: 1.9 us a launch in a chain of them.
+// front.  Bound by memory: every byte is read once and written once; 1,000 pages of twelve tensors, 197 MB in and out, 36.6 us, 5.4
+// TB/s.  One page and a state slot: 2.7 us a launch in a chain of them.
 #include <exception>
 #include <vector>
 
@@ -20,15 +20,17 @@ struct Piece {
 };
 struct Copies {
   const Piece* pieces;
-  int n_groups;
+  int n_groups, last;                                         // last: of the call's launches
   int first_piece[MAX_GROUPS + 1], first_pair[MAX_GROUPS + 1];
   unsigned first_unit[MAX_GROUPS + 1];                        // a unit: a pair and a piece
   int2 pairs[MAX_PAIRS];                                      // (src, dst)
 };
 static_assert(sizeof(Copies) <= 4096, "the arguments of a launch");
 
+// Only another launch of the same call may start early: kernels read what earlier steps left in pages and slots ahead of their wait, and
+// the rows that are written here are such.
 __global__ void __launch_bounds__(256) row_copies_kernel(const __grid_constant__ Copies c) {
-  pdl_trigger();
+  if (!c.last) pdl_trigger();
   const int lane = threadIdx.x & 31;
   const unsigned unit = blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   if (unit >= c.first_unit[c.n_groups]) return;
@@ -54,6 +56,7 @@ __global__ void __launch_bounds__(256) row_copies_kernel(const __grid_constant__
   } else {
     for (int i = lane; i < (int)p.bytes; i += 32) dst[i] = src[i];
   }
+  if (c.last) __threadfence();                                 // (in place for the whole GPU before this block ends)
 }
 
 // Ids within the group, no destination twice, none that is a source too.
@@ -110,6 +113,8 @@ GB_API int gb_row_copies(const long long* w) {
     if (rc != GB_OK) return rc;
   }
   int launched = 0;
+  long long to_copy = 0;                                       // pairs (of groups that have pieces) that no launch has yet
+  for (int g = 0; g < n_groups; ++g) to_copy += n_pieces[g] > 0 ? n_pairs[g] : 0;
   int g0 = 0, done = 0;                                        // group and pair of it that come next
   while (g0 < n_groups) {
     // as many pairs as the arguments hold, group after group
@@ -129,6 +134,7 @@ GB_API int gb_row_copies(const long long* w) {
       used += take;
       done += take;
       units += (long long)take * n_pieces[g];
+      to_copy -= n_pieces[g] > 0 ? take : 0;
       if (done == n_pairs[g]) {
         ++g0;
         done = 0;
@@ -139,6 +145,7 @@ GB_API int gb_row_copies(const long long* w) {
     c.first_unit[n_groups] = (unsigned)units;
     if (units > 0x7fffffffll) GB_FAIL(GB_ERR_ARG, "gb_row_copies: %lld pieces in one launch", units);
     if (units == 0) continue;
+    c.last = to_copy == 0;
     gb_launch(row_copies_kernel, dim3((unsigned)((units + 7) / 8)), dim3(256), 0, stream, c);
     GB_CHECK_LAUNCH("gb_row_copies");
     ++launched;
