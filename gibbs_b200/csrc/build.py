@@ -26,7 +26,7 @@ HERE = Path(__file__).resolve().parent
 # it computes in bfloat16; "runtime" holds no kernels: it walks a step's list of operations
 # and calls into the others; "hybrid" is built when a model has a part that launches from it.
 LIBRARIES = {
-    "core": ["errors.cu", "elementwise.cu", "gemm_simt.cu", "conv.cu", "attention.cu", "sampling.cu"],
+    "core": ["errors.cu", "elementwise.cu", "gemm_simt.cu", "conv.cu", "attention.cu", "sampling.cu", "row_copies.cu"],
     "tensorcore": ["errors.cu", "gemm_tc.cu", "gemm_tc_decode.cu", "attention_tc.cu", "attention_tcgen05.cu"],
     "runtime": ["errors.cu", "step_plan.cu"],
     # layer norms, clamped gated units, latent, gated and sigmoid attention, state-space, delta-rule and linear recurrences, residual
@@ -35,7 +35,7 @@ LIBRARIES = {
     "hybrid": ["errors.cu", "norms.cu", "latent_attention.cu", "latent_attention_tc.cu", "gated_attention.cu", "gated_attention_tc.cu", "gated_attention_tcgen05.cu",
                "sigmoid_attention_tc.cu", "ssm.cu", "selective_scan.cu", "delta_rule.cu", "delta_chunks.cu", "linear_scan.cu", "streams.cu", "moe.cu",
                "moe_tc.cu"],
-    # the 8-bit paged cache: storing, attention, and copies of rows of any cache (forked requests)
+    # the 8-bit paged cache: storing, attention, and copies of its rows (as in "core", for callers of this library alone)
     "kv8": ["errors.cu", "kv8_store.cu", "kv8_attention.cu", "kv8_attention_tcgen05.cu", "kv8_call.cu", "row_copies.cu"],
 }
 

@@ -214,7 +214,10 @@ class Engine:
             ops.ensure_built(["kv8"])
         self.cache = CacheManager(model.entry_needs(), n_pages, page_size, self.max_requests, model.rt.dtype,
                                   self.device, self.max_context, guard=guard_cache, kv_dtype=kv_dtype)
-        self._row_copies = None
+        # What forks copy with: made here, so that the first one in the middle of serving loads and uploads nothing.
+        tensors = self.cache.copied_tensors()
+        self._forkable = len(tensors) <= ops.row_copies.MAX_GROUPS
+        self._row_copies = ops.RowCopies(tensors) if tensors and self._forkable else None
         self.vocab_size = model.vocab_size
         self.status = ops.device_status(self.device)
         self.builder = StepBuilder(self.cache, self.device, self.max_requests, self.max_step_tokens, self.status)
@@ -260,12 +263,11 @@ class Engine:
         """Open ``new_id`` where ``request_id`` stands: both go on from the same tokens, each on its own.  Full pages are
         shared; the page that both will write on and the state of layers that keep some are copied, in one launch.  Raises
         OutOfPages or OutOfSlots, and changes nothing, when the pools cannot hold the new request."""
-        if self._row_copies is None:
-            tensors = self.cache.copied_tensors()
-            self._row_copies = ops.RowCopies(tensors) if tensors else False
+        if not self._forkable:
+            raise StepError(f"a fork copies {ops.row_copies.MAX_GROUPS} groups of pages and slots at most; this cache has more")
         pairs = self.cache.fork(request_id, new_id)
         try:
-            if self._row_copies and any(pairs):
+            if any(pairs):
                 self._row_copies.copy(pairs)
         except BaseException:
             self.cache.close(new_id)

@@ -10,7 +10,7 @@ import torch
 from . import _launched, raw_stream
 from .library import KernelError, check, library
 
-LIBRARY = "kv8"
+LIBRARY = "core"                 # (an engine forks whatever its cache is held in)
 MAX_GROUPS = 16
 
 
