@@ -46,13 +46,14 @@ Several answers to one prompt (``submit(..., samples=n)``).  The first request
 runs the prompt; the others wait with it, and in the step that ends the prompt
 each takes its first token from the same logits and is forked from the first
 (``Engine.fork``: full pages shared, the last one and the state copied).  When
-some find no slot or page then, or the first is cancelled or fails, the next of
+some find no slot or page then, or their fork raises, or the first is cancelled or fails, the next of
 them runs the prompt again for those that are left; a request's seed and the
 number of tokens it has drawn decide its picks, whoever ran its prompt.
 """
 from __future__ import annotations
 
 import time
+import warnings
 from collections import deque
 from dataclasses import dataclass, field
 from enum import Enum
@@ -283,12 +284,16 @@ class Scheduler:
         self.waiting.extendleft(reversed(live + [f for f in followers if f.cancelled]))
 
     def _join(self, leader: Sequence_, follower: Sequence_) -> bool:
-        """Fork ``follower`` from ``leader``, which has just run their prompt; False when it cannot be."""
+        """Fork ``follower`` from ``leader``, which has just run their prompt; False when it cannot be, for want of room or
+        because the fork raised: it then runs the prompt itself, and this step's tokens are emitted whatever happened here."""
         if not hasattr(self.engine, "fork") or follower.cancelled or len(self.running) >= self.max_running:
             return False
         try:
             self.engine.fork(leader.id, follower.id)
         except (OutOfSlots, OutOfPages):
+            return False
+        except Exception as e:
+            warnings.warn(f"a fork failed, its prompt is run again: {e}", RuntimeWarning)
             return False
         follower.state, follower.admitted, follower.fed = SeqState.RUNNING, self._admissions, len(follower.prompt)
         self._admissions += 1
