@@ -137,6 +137,7 @@ class Sequence_:
     preemptions: int = 0
     cancelled: bool = False
     followers: list = field(default_factory=list)   # further answers to this prompt that wait for it to have been run
+    leader: Optional["Sequence_"] = field(default=None, repr=False, compare=False)      # whose follower this is
 
     @property
     def tokens(self) -> list:
@@ -220,6 +221,7 @@ class Scheduler:
         self.waiting: deque = deque()
         self.running: list = []
         self.sequences: dict = {}
+        self._gave_up: list = []                    # followers cancelled since the last step
         self._next_id = 0
         self._admissions = 0
         self.steps = 0
@@ -239,6 +241,7 @@ class Scheduler:
                 seq = self.sequences[sid]
                 self.waiting.remove(seq)
                 leader.followers.append(seq)
+                seq.leader = leader
             return ids
         params = params or SamplingParams()
         prompt = [int(t) for t in prompt] or [1]
@@ -257,7 +260,10 @@ class Scheduler:
 
     def cancel(self, sid: int) -> None:
         """The client gave up: the request ends at the next step."""
-        self.sequences[sid].cancelled = True
+        seq = self.sequences[sid]
+        seq.cancelled = True
+        if seq.leader is not None:
+            self._gave_up.append(seq)
 
     def has_work(self) -> bool:
         return bool(self.waiting or self.running or self._inflight is not None)
@@ -271,17 +277,33 @@ class Scheduler:
             self.waiting.remove(seq)
         seq.state, seq.finish, seq.error = SeqState.FINISHED, reason, error
         out.finished.append((seq.id, reason))
-        self._release(seq)
+        self._release(seq, out)
 
-    def _release(self, seq: Sequence_) -> None:
+    def _end_followers(self, out: StepOutput) -> None:
+        """Those that were cancelled while they wait for another request to run their prompt."""
+        gave_up, self._gave_up = self._gave_up, []
+        for seq in gave_up:
+            if seq.leader is not None:
+                seq.leader.followers = [f for f in seq.leader.followers if f is not seq]
+                seq.leader = None
+                self._finish(seq, FinishReason.CANCELLED, out)
+
+    def _release(self, seq: Sequence_, out: StepOutput) -> None:
         """What still waits for this request's prompt: the first of them runs it next, and the others wait for that one (for an
         engine that cannot fork, every one runs it)."""
         followers, seq.followers = seq.followers, []
+        for f in followers:
+            f.leader = None
         live = [f for f in followers if not f.cancelled]
         if live and hasattr(self.engine, "fork"):
             live[0].followers = live[1:]
+            for f in live[1:]:
+                f.leader = live[0]
             live = live[:1]
-        self.waiting.extendleft(reversed(live + [f for f in followers if f.cancelled]))
+        self.waiting.extendleft(reversed(live))
+        for f in followers:
+            if f.cancelled:
+                self._finish(f, FinishReason.CANCELLED, out)
 
     def _join(self, leader: Sequence_, follower: Sequence_) -> bool:
         """Fork ``follower`` from ``leader``, which has just run their prompt; False when it cannot be, for want of room or
@@ -295,6 +317,7 @@ class Scheduler:
         except Exception as e:
             warnings.warn(f"a fork failed, its prompt is run again: {e}", RuntimeWarning)
             return False
+        follower.leader = None
         follower.state, follower.admitted, follower.fed = SeqState.RUNNING, self._admissions, len(follower.prompt)
         self._admissions += 1
         self.running.append(follower)
@@ -372,6 +395,7 @@ class Scheduler:
     def step(self) -> StepOutput:
         out = StepOutput()
         self.steps += 1
+        self._end_followers(out)
         prev = self._inflight
         if prev is not None:
             # the next decode step goes out on the device's ids before the host reads this one's
@@ -467,7 +491,7 @@ class Scheduler:
                 picks = [f for f in s.followers if any(f is x for x in samplers)]
                 kept = [f for f in picks if self._join(s, f)]
                 s.followers = [f for f in s.followers if not any(f is x for x in kept)]
-                self._release(s)                    # (those that found no place; their token is picked again)
+                self._release(s, out)               # (those that found no place; their token is picked again)
         if pending is not None:
             self._inflight = _InFlight(samplers, pending, t0, n_prefill, n_decode)
             out.active_sequences = len(self.running)

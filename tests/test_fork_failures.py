@@ -1,4 +1,4 @@
-"""Several answers to a prompt where forks raise."""
+"""Several answers to a prompt where forks raise, and where a client goes while it waits."""
 import pytest
 
 from fake_engine import FakeEngine
@@ -50,3 +50,59 @@ def test_a_fork_that_raises_beside_other_requests():
     sched.run(max_steps=200)
     assert not sched.has_work() and [len(sched.sequences[i].output) for i in [other] + ids] == [8, 3, 3]
     eng.cache.check()
+
+
+# ---------------------------------------------------------------------------------------------------
+@pytest.mark.parametrize("overlap", [False, True])
+def test_an_answer_that_waits_for_its_prompt_ends_at_the_step_after_its_cancellation(overlap):
+    """Wherever the request that runs the prompt is: running it, or waiting for a place behind another request."""
+    params = SamplingParams(max_new_tokens=5, seed=1)
+    want, _, _ = _answers(FakeEngine(), [4, 5, 6, 7, 8], 3, params, samples=False)
+    for places, before in ((8, 0), (8, 1), (1, 0), (1, 2)):
+        eng = ForkingEngine()
+        sched = Scheduler(eng, SeededSampler(eng.vocab), max_batch_tokens=2, max_running=places, overlap=overlap)
+        if places == 1:
+            sched.submit([1], SamplingParams(max_new_tokens=12, seed=0))
+        ids = sched.submit([4, 5, 6, 7, 8], params, samples=3)
+        for _ in range(before):
+            sched.step()
+        sched.cancel(ids[1])
+        out = sched.step()
+        assert (ids[1], FinishReason.CANCELLED) in out.finished
+        assert sched.sequences[ids[1]].finish == FinishReason.CANCELLED
+        sched.cancel(ids[1])                                       # (again: nothing)
+        outs = sched.run(max_steps=300)
+        assert not sched.has_work() and all(i != ids[1] for o in outs for i, _ in o.finished + o.emitted)
+        assert [sched.sequences[i].output for i in ids] == [want[0], [], want[2]]
+        eng.cache.check()
+
+
+def test_an_answer_that_was_cancelled_takes_no_row_of_logits():
+    """Two of five answers are cancelled between the steps of a prompt; the engine has room for three rows beside the first's."""
+    eng = ForkingEngine()
+    eng.max_step_tokens = 3
+    sampler = SeededSampler(eng.vocab)
+    sched = Scheduler(eng, sampler, max_batch_tokens=3)
+    ids = sched.submit([4, 5, 6, 7, 8], SamplingParams(max_new_tokens=4, seed=1), samples=5)
+    sched.step()
+    sched.cancel(ids[1]), sched.cancel(ids[2])
+    sched.step()                                                   # (the prompt's last tokens)
+    assert sampler.rows[-1] == 3 and eng.events.count("fork") == 2
+    sched.run(max_steps=100)
+    assert [len(sched.sequences[i].output) for i in ids] == [4, 0, 0, 4, 4]
+
+
+def test_all_that_wait_are_cancelled_or_the_leader_with_one_of_them():
+    for gone in ((1, 2), (0, 1), (0, 1, 2)):
+        eng = ForkingEngine()
+        sched = Scheduler(eng, SeededSampler(eng.vocab), max_batch_tokens=2)
+        ids = sched.submit([4, 5, 6, 7, 8], SamplingParams(max_new_tokens=4, seed=1), samples=3)
+        sched.step()
+        for i in gone:
+            sched.cancel(ids[i])
+        out = sched.step()
+        assert sorted(i for i, _ in out.finished) == sorted(ids[i] for i in gone)
+        sched.run(max_steps=100)
+        assert not sched.has_work()
+        assert [sched.sequences[i].finish for i in ids] == [FinishReason.CANCELLED if i in gone else FinishReason.LENGTH for i in range(3)]
+        assert all(f == g.pool.size for f, g in zip(eng.cache.free_pages(), eng.cache.groups))
