@@ -233,7 +233,7 @@ class Scheduler:
         if samples < 1:
             raise ValueError(f"{samples} samples")
         if samples > 1:
-            params = params or SamplingParams()
+            prompt, params = list(prompt), params or SamplingParams()
             each = [params if params.seed is None else SamplingParams(**{**params.__dict__, "seed": params.seed + i}) for i in range(samples)]
             ids = [self.submit(prompt, p) for p in each]
             leader = self.sequences[ids[0]]

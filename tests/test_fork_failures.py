@@ -106,3 +106,18 @@ def test_all_that_wait_are_cancelled_or_the_leader_with_one_of_them():
         assert not sched.has_work()
         assert [sched.sequences[i].finish for i in ids] == [FinishReason.CANCELLED if i in gone else FinishReason.LENGTH for i in range(3)]
         assert all(f == g.pool.size for f, g in zip(eng.cache.free_pages(), eng.cache.groups))
+
+
+def test_a_prompt_given_as_an_iterator():
+    """(As for one answer: the prompt is gone through once.)"""
+    params = SamplingParams(max_new_tokens=4, seed=1)
+    want, _, _ = _answers(ForkingEngine(), [4, 5, 6, 7, 8], 3, params)
+    assert _answers(ForkingEngine(), iter([4, 5, 6, 7, 8]), 3, params)[0] == want
+
+
+def test_a_prompt_that_is_refused_leaves_nothing_behind():
+    eng = ForkingEngine()
+    sched = Scheduler(eng, SeededSampler(eng.vocab))
+    with pytest.raises(ValueError):
+        sched.submit([1] * (eng.max_context + 1), SamplingParams(seed=0), samples=3)
+    assert not sched.has_work() and not sched.sequences
