@@ -29,20 +29,21 @@ def pages_for(model: CausalLM, page_size: int, max_running: int, ctx: int, memor
     """Pages to allocate per group: enough for ``max_running`` requests of
     ``ctx`` tokens, or what ``memory_fraction`` of the free device memory
     holds, whichever is smaller."""
-    per_token = 0
+    per_token = scales = 0                           # bytes a position, and a page of an 8-bit cache beside
     kv_bytes = 1 if parse_cache_dtype(cache_dtype) is not None else 2 if model.rt.dtype == torch.bfloat16 else 4
     for needs, reads in model.entry_needs():
         if reads is None:
             for need in needs:
                 if hasattr(need, "kv_heads"):
                     per_token += need.kv_heads * (need.head_dim + need.value_dim) * kv_bytes
+                    scales += need.kv_heads * 8 if kv_bytes == 1 else 0
                 elif hasattr(need, "width"):             # one plain row per position (PagedRows)
                     per_token += need.width * (2 if model.rt.dtype == torch.bfloat16 else 4)
     want = max_running * -(-ctx // page_size)
     if per_token == 0:
         return 1
     free, _ = torch.cuda.mem_get_info(model.rt.device)
-    by_memory = int(free * memory_fraction) // (per_token * page_size)
+    by_memory = int(free * memory_fraction) // (per_token * page_size + scales)
     return max(1, min(want, by_memory))
 
 
