@@ -951,8 +951,9 @@ GB_OP(gb_op_kv8_attention) {
   p.window = a[16] > 0x3fffffff ? 0 : (int)a[16];               // (one that no context reaches is none, and sums with it stay in 32 bits)
   p.scale_log2 = (float)(f[0] * 1.4426950408889634);
   p.status = ctx->status;
-  if (p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads != 0 || p.hd <= 0 || p.hd % 8 != 0 || p.hd > 256 || p.page_size <= 0)
-    GB_FAIL(GB_ERR_ARG, "kv8_attention: %d heads, %d kv heads, head_dim %d, pages of %d: head sizes are multiples of 8 up to 256",
+  if (p.heads <= 0 || p.kv_heads <= 0 || p.heads % p.kv_heads != 0 || p.hd <= 0 || p.hd % 8 != 0 || p.hd > 256 || p.page_size <= 0 ||
+      (long long)p.page_size * p.hd > 0x7fffffff)
+    GB_FAIL(GB_ERR_ARG, "kv8_attention: %d heads, %d kv heads, head_dim %d, pages of %d: head sizes are multiples of 8 up to 256, a page's rows of a head fewer than 2^31 entries",
             p.heads, p.kv_heads, p.hd, p.page_size);
   if (dtype != GB_F32 && dtype != GB_BF16) GB_FAIL(GB_ERR_ARG, "kv8_attention: q and out are float32 or bfloat16");
   if (!isfinite(p.scale_log2)) GB_FAIL(GB_ERR_ARG, "kv8_attention: a scale of %g", f[0]);

@@ -511,8 +511,9 @@ GB_OP(gb_op_kv8_store) {
   p.splits = (flags & GB_OP_TAKES_PARTIALS) && ctx->part != nullptr ? ctx->part_splits : 0;
   p.part_bias = ctx->part_bias;
   p.part_stride = 0;
-  if (p.heads <= 0 || p.kv_heads <= 0 || p.hd <= 0 || p.hd % 8 != 0 || p.hd > 256 || p.page_size <= 0)
-    GB_FAIL(GB_ERR_ARG, "kv8_store: %d heads, %d kv heads, head_dim %d, pages of %d: head sizes are multiples of 8 up to 256",
+  if (p.heads <= 0 || p.kv_heads <= 0 || p.hd <= 0 || p.hd % 8 != 0 || p.hd > 256 || p.page_size <= 0 ||
+      (long long)p.page_size * p.hd > 0x7fffffff)
+    GB_FAIL(GB_ERR_ARG, "kv8_store: %d heads, %d kv heads, head_dim %d, pages of %d: head sizes are multiples of 8 up to 256, a page's rows of a head fewer than 2^31 entries",
             p.heads, p.kv_heads, p.hd, p.page_size);
   if (dtype != GB_F32 && dtype != GB_BF16) GB_FAIL(GB_ERR_ARG, "kv8_store: rows are float32 or bfloat16");
   if (p.rotary != nullptr && (p.rotary_dim < 0 || p.rotary_dim > p.hd || p.rotary_dim % 2 != 0))

@@ -26,3 +26,21 @@ def test_pages_by_memory_count_the_scales(monkeypatch, page, kv_heads, hd):
             m = CacheManager(needs, pages, page, 1, torch.bfloat16, "cpu", 1 << 20, kv_dtype=kv_dtype)
             return sum(t.numel() * t.element_size() for g in m.copied_tensors() for t in g)
         assert size(n) <= free * 0.5 < size(n + 1)
+
+
+@pytest.mark.parametrize("operation", [0, 1])
+@pytest.mark.parametrize("page,hd", [(1 << 30, 8), (1 << 25, 64), ((1 << 30) + 16, 64), ((1 << 31) - 16, 8), (1 << 28, 8)])
+def test_pages_whose_rows_pass_32_bits_are_refused(operation, page, hd):
+    """A page of a head with 2^31 entries or more, before anything is launched (or counted towards)."""
+    from gibbs_b200.ops.library import library
+    lib = library("kv8")
+    lib.gb_kv8_run.argtypes, lib.gb_kv8_run.restype = [ctypes.c_char_p], ctypes.c_int
+    lib.gb_last_error.restype = ctypes.c_char_p
+    heads, kv_heads, bf16 = 4, 2, 1
+    if operation == 0:
+        operands = [0, 8 * hd, bf16, 0, 0, 0, 0, 0, 0, 16, 16, 16, 16, 1, page, heads, kv_heads, hd, 0, 1]
+    else:
+        operands = [0, 4 * hd, bf16, 0, 4 * hd, 16, 16, 16, 16, 1, page, heads, kv_heads, hd, 0, 1, 0, 0, 0, 0]
+    words = struct.pack("=18qd20q", operation, 0, 0, 1, 1, 0, 1, 1, 1, 0, 0, 0, 0, 0, 0, 0, 0, 0, 0.125, *operands)
+    assert lib.gb_kv8_run(words) < 0
+    assert b"pages of" in lib.gb_last_error()
