@@ -17,7 +17,7 @@ MAX_GROUPS = 16
 class RowCopies:
     """Row copies within ``groups`` of tensors: the tensors of a group (K and V pages of every layer and their scales, say)
     have one number of rows, and what is copied in one is copied in all.  A tensor's rows are contiguous; the rows may be
-    strided.  Made once for a cache; holds the tensors."""
+    strided; groups share no memory.  Made once for a cache; holds the tensors."""
 
     def __init__(self, groups: Sequence[Sequence[torch.Tensor]]):
         self.groups = [list(g) for g in groups]
@@ -66,15 +66,13 @@ class RowCopies:
                 keep.append(p)
                 words += (p.data_ptr(), len(p))
             else:
-                flat = [v for pair in p for v in pair]
                 try:
+                    flat = [v for src, dst in p for v in (src, dst)]
                     a = (ctypes.c_int * len(flat)).from_buffer_copy(struct.pack(f"={len(flat)}i", *flat)) if flat else None
-                except struct.error as e:
-                    raise KernelError(f"row copies: pairs of group {i} are 32-bit integers ({e})") from None
-                if len(flat) != 2 * len(p):
-                    raise KernelError(f"row copies: pairs of group {i} are (src, dst)")
+                except (struct.error, TypeError, ValueError) as e:
+                    raise KernelError(f"row copies: pairs of group {i} are (src, dst), 32-bit integers ({e})") from None
                 keep.append(a)
-                words += (0 if a is None else ctypes.addressof(a), len(p))
+                words += (0 if a is None else ctypes.addressof(a), len(flat) // 2)
         rc = self._run(struct.pack(self._format, self._table, raw_stream(self.device), len(self.groups), *words, *self._sizes))
         if rc < 0:
             check(library(LIBRARY), rc)

@@ -57,3 +57,17 @@ def test_copies_attention_and_convolution_one_right_behind_the_other():
     for _ in range(4):
         assert all(torch.equal(a, b) for a, b in zip(run(lambda: None), want))
     assert int(hints.status.item()) == 0
+
+
+@pytest.mark.parametrize("pairs", [[(0, 1, 2), (3,)], [(0, 1), (2,)], [(0, 1, 2, 3)], [(), (0, 1, 2, 3)], [0, 1], [("0", "1")], [(0.0, 1.0)], [(None, 1)],
+                                   [[[0, 1], [2, 3]]]])
+def test_pairs_that_are_not_pairs_are_refused(pairs):
+    from gibbs_b200.ops import KernelError, RowCopies
+    t = torch.arange(40, device=DEV).float().view(10, 4)
+    before, copies = t.clone(), RowCopies([[t], [t.clone()]])
+    for given in ([pairs, []], [[], pairs]):
+        with pytest.raises(KernelError, match="row copies"):
+            copies.copy(given)
+    assert torch.equal(t, before)
+    assert copies.copy([[], [[1, 0]]]) == 1 and copies.copy([[(3, 2)], []]) == 1
+    assert torch.equal(t[2], t[3])
