@@ -39,3 +39,29 @@ def test_a_cache_of_more_kinds_of_pages_than_a_fork_copies(tmp_path, monkeypatch
         eng.fork("a", "b")
     assert not eng.is_live("b") and eng.length("a") == 3
     eng.cache.check()
+
+
+@pytest.mark.parametrize("cache_dtype", [None, "float8_e4m3"])
+@pytest.mark.parametrize("name,dtype", [("A", "float32"), ("B", "bfloat16"), ("C", "bfloat16")])
+def test_one_place_wanted_twice_beside_a_token_whose_logits_nobody_wants(tmp_path, name, dtype, cache_dtype):
+    """As many tokens, requests and wanted rows as a decode step of that size has, but other rows: with graphs (which such a step then
+    is recorded into, or replayed from) and without, before and after decode steps of that size."""
+    from gibbs_b200 import Engine, StepEntry, load_model
+    model = load_model(make_folder(tmp_path, name, stored=torch.bfloat16 if dtype == "bfloat16" else torch.float32), dtype=dtype, device="cuda:0")
+    tokens = random_ids(2, 20, TINY[name][0]["vocab_size"])
+    got = []
+    for graphs in (False, True):
+        eng = Engine(model, n_pages=32, page_size=16, max_requests=4, max_step_tokens=128, cache_dtype=cache_dtype, use_graphs=graphs)
+        for r in "ab":
+            eng.open(r)
+        rows = [eng.step([StepEntry("a", tokens[:1], [0, 0]), StepEntry("b", tokens[1:2], [])]).clone()]
+        rows.append(eng.step([StepEntry("a", tokens[2:3], [0]), StepEntry("b", tokens[3:4], [0])]).clone())
+        rows.append(eng.step([StepEntry("a", tokens[4:5], []), StepEntry("b", tokens[5:6], [0, 0])]).clone())
+        rows.append(eng.step([StepEntry("a", tokens[6:7], [0]), StepEntry("b", tokens[7:8], [0])]).clone())
+        eng.fork("b", "c")
+        rows.append(eng.step([StepEntry("c", tokens[8:9], [0]), StepEntry("b", tokens[8:9], [0])]).clone())
+        eng.check_status()
+        assert torch.equal(rows[0][0], rows[0][1]) and torch.equal(rows[2][0], rows[2][1]) and torch.equal(rows[4][0], rows[4][1])
+        assert not torch.equal(rows[1][0], rows[1][1])
+        got.append(rows)
+    assert all(torch.equal(a, b) for a, b in zip(*got))
