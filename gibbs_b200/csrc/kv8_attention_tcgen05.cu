@@ -174,6 +174,9 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
     abort_flag = 0;
     fence_barrier_init();
   }
+  // All of tensor memory, but not while waiting for another kernel: a CTA of that one which has started and not taken its columns yet
+  // would wait for these.
+  pdl_wait();
   if (warp == 11) {
     tmem_alloc(&tmem_slot, 512);
     tmem_relinquish();
@@ -184,7 +187,6 @@ __global__ void __launch_bounds__(THREADS, 1) kv8_attention_tcgen05_kernel(const
   const uint32_t tmem = tmem_slot;
   const uint32_t tmem_s[2] = {tmem, tmem + KEYS}, tmem_o[2] = {tmem + 2 * KEYS, tmem + 2 * KEYS + HD};
   const uint32_t tmem_p[2] = {C::APART ? tmem + 2 * KEYS + 2 * HD : tmem, C::APART ? tmem + 2 * KEYS + 2 * HD + KEYS / 2 : tmem + KEYS};
-  pdl_wait();
 
   if (warp >= 8 && warp < 11) {
     // ---- K and V: pages -> f16 tiles ----

@@ -155,3 +155,40 @@ def test_a_launch_without_work_ends_behind_the_kernel_in_front():
         torch.cuda.synchronize()
         assert torch.equal(got, kv8.paged_attention(q, heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, out, step))
         assert int(step.status.item()) == 0
+
+
+@pytest.mark.parametrize("way", ["256 rows, 64", "256 rows, 128", "256 rows beside 8"])
+def test_products_store_and_attention_on_two_streams_without_a_pause(way):
+    """Layers' worth of (product, store, attention, product), whose kernels share the SMs' tensor memory, in one stream and in two at
+    once: every run ends and gives the same bits."""
+    from gibbs_b200 import ops
+    from gibbs_b200.ops import kv8
+    dtype, heads, kv_heads, hd, page, portions = WAYS[way]
+    n, behind, wide = sum(portions), [(37 * i) % 90 for i in range(len(portions))], (heads + 2 * kv_heads) * hd
+    gen = torch.Generator().manual_seed(5)
+    n_pages, bt = tables(portions, behind, page, random.Random(1))
+    bt, step = bt.to(DEV), step_of(portions, behind)
+    w_in, w_out = ((torch.randn(a, b, generator=gen) * b ** -0.5).to(dtype).to(DEV) for a, b in ((wide, 512), (512, heads * hd)))
+    x0, clean = torch.randn(n, 512, generator=gen).to(dtype).to(DEV), make_pages(n_pages, kv_heads, page, hd, gen)
+
+    def layers():
+        pages, x = kv8.Pages(*(t.clone() for t in clean.tensors())), x0
+        for _ in range(12):
+            rows, q, out, y = (torch.empty(n, c, dtype=dtype, device=DEV) for c in (wide, heads * hd, heads * hd, 512))
+            ops.linear(x, w_in, None, rows)
+            kv8.qk_norm_rope_store(rows, q, heads, kv_heads, hd, None, None, 1e-5, None, 0, False, step, bt, pages)
+            kv8.paged_attention(q, heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, out, step)
+            x = ops.linear(out, w_out, None, y)
+        return x
+
+    want = layers()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for s in streams:
+            with torch.cuda.stream(s):
+                got.append(layers())
+        torch.cuda.synchronize()
+        assert all(torch.equal(g, want) for g in got) and not bool(want.isnan().any())
+    assert int(step.status.item()) == 0
