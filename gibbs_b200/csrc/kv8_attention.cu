@@ -966,8 +966,12 @@ GB_OP(gb_op_kv8_attention) {
   // Requests of more than FEW rows go to tcgen05, which takes 256 rows at a time; they have to lie on 16-byte boundaries.
   const bool wide = mma && (long long)p.step.max_q * group > FEW && group <= 64 && p.ldo % 8 == 0 && ((uintptr_t)p.out & 15) == 0;
   p.few = 0x7fffffff;
-  if (wide && p.step.n_requests == 1) {
-    p.few = 0;                                                 // (all of it, whatever it brings)
+  // Where no request can have few rows (the shortest brings at least what the longest leave of the step's tokens) there is nothing for the
+  // launch in front, which would be waited for: 8 requests of 16 tokens over 2,000 keys, 32 / 8 heads of 64, 32 us without it and 34
+  // with it, two of 16 over 4,000 keys with heads of 128 33 and 40.
+  const long long shortest = p.step.n_tokens - (p.step.n_requests - 1ll) * p.step.max_q;
+  if (wide && (p.step.n_requests == 1 || shortest * group > FEW)) {
+    p.few = 0;                                                 // (all of it, whatever a request brings)
     const int rc = kv8_attention_tcgen05(p, ctx->stream);
     return rc == GB_OK ? 1 : rc;
   }

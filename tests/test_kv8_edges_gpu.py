@@ -192,3 +192,31 @@ def test_products_store_and_attention_on_two_streams_without_a_pause(way):
         torch.cuda.synchronize()
         assert all(torch.equal(g, want) for g in got) and not bool(want.isnan().any())
     assert int(step.status.item()) == 0
+
+
+@pytest.mark.parametrize("hd,page", [(64, 16), (128, 64)])
+@pytest.mark.parametrize("portions", [[20, 20, 20], [13, 60, 60], [12, 60, 60], [1, 60, 60], [60, 0, 60], [13, 14, 13]])
+def test_steps_at_the_border_of_what_one_launch_takes(portions, hd, page):
+    """Groups of four heads: 13 tokens are more than 48 rows and 12 are not.  Each request gets what it gets alone, to a bfloat16's last
+    place of what its sums go over; rows behind the tokens are left, also where a step counts more tokens than its requests bring."""
+    from gibbs_b200.ops import kv8
+    heads, kv_heads, behind = 32, 8, [70, 300, 5]
+    gen = torch.Generator().manual_seed(6)
+    n_pages, bt = tables(portions, behind, page, random.Random(1))
+    pages, bt = make_pages(n_pages, kv_heads, page, hd, gen), bt.to(DEV)
+    n = sum(portions)
+    q = torch.randn(n + 9, heads * hd, generator=gen).to(torch.bfloat16).to(DEV)
+    for more in (0, 9):
+        step = step_of(portions, behind)
+        step.n_tokens += more
+        out = kv8.paged_attention(q, heads, kv_heads, hd, pages, bt, hd ** -0.5, 0, torch.full_like(q, 7.0), step)
+        assert bool((out[n:] == 7.0).all()) and int(step.status.item()) == 0
+        at = 0
+        for r, (p, b) in enumerate(zip(portions, behind)):
+            if not p:
+                continue
+            alone = kv8.paged_attention(q[at:at + p], heads, kv_heads, hd, pages, bt[r:r + 1], hd ** -0.5, 0, torch.empty_like(q[at:at + p]), step_of([p], [b]))
+            # (weights in f16 under another running maximum: 2^-11 of them each, twice; and the output's rounding, twice)
+            size = pages.dequantized()[1][bt[r, :-(-(p + b) // page)].long()].abs().amax().item()
+            assert bool(((out[at:at + p].float() - alone.float()).abs() <= 2 * 2.0 ** -11 * size + 2 * 2.0 ** -8 * alone.float().abs()).all())
+            at += p
