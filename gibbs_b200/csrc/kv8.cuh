@@ -32,7 +32,8 @@ __device__ __forceinline__ float scale_for(float amax) {
   const int e = (bits >> 23) - 127 - 8 + ((bits & 0x7fffff) > 0x600000 ? 1 : 0);
   return pow2(e < MIN_EXP ? MIN_EXP : e);
 }
-// 1 / scale of a power of two within the exponents above (0 for anything that is not one: a scale nobody set).
+// 1 / scale of a power of two within the exponents above, by its exponent alone.  (Of 0, a scale nobody set or no page: 2^127, which only
+// weights of 0 meet.)
 __device__ __forceinline__ float inverse(float scale) {
   const int bits = __float_as_int(scale);
   return __int_as_float((254 << 23) - (bits & 0x7f800000));

@@ -13,7 +13,7 @@
 // The two row tiles take turns: while one is in its softmax the other's products run, and both use the same converted K and V.  (Products
 // issued as either tile is ready, without that order: 48 us against 47 at 2,048 tokens, 345 against 327 at 8,192.)
 //
-// 2,048 tokens, 32 / 8 heads of 64: 44.8 us, 384 TFLOP/s; 8,192 tokens, 16 / 4 heads of 128: 315 us, 873 TFLOP/s.  What bounds it, from
+// 2,048 tokens, 32 / 8 heads of 64: 45.1 us, 381 TFLOP/s; 8,192 tokens, 16 / 4 heads of 128: 316 us, 870 TFLOP/s.  What bounds it, from
 // copies that left work out when it took 47 and 327: heads of 64 take 45 us without the 2^x, 40 without any softmax, 34 without conversion and loads either, so it is
 // the hand-overs of a key tile (scores to registers, weights back, product) and a CTA's beginning and end; heads of 128 take 301 us
 // without conversion, 296 without softmax and 229 without both.  The special-function unit is at 37 % (a share of the 2^x by a
@@ -709,7 +709,7 @@ int launch(const Attn& p, long long tiles, long long keys, cudaStream_t stream) 
   // CTAs that share a tile's keys: as many as the SMs hold at a time, each with four key tiles at least.  `tiles` is an upper bound that
   // counts one for every request; how many there are is estimated from the longest portion and the mean of the others, which are
   // taken to be as long as their mean, or, where that is few rows, to be single tokens and a portion that has the rest of them.  (Without
-  // the others 8 requests of 16 tokens behind 4,000 keys, 32 / 8 heads of 64, take 79 us, by eight CTAs a tile; with them 52, by two.)
+  // the others 8 requests of 16 tokens behind 4,000 keys, 32 / 8 heads of 64, take 79 us, by eight CTAs a tile; with them 49, by two.)
   const long long two = 2 * (ROWS / (p.heads / p.kv_heads)), others = p.step.n_requests - 1, rest = p.step.n_tokens - p.step.max_q;
   const bool alike = others > 0 && rest * (p.heads / p.kv_heads) > others * p.few;
   const long long of_others = alike ? others * ((rest / others + two - 1) / two) : (rest + two - 1) / two;
